@@ -942,13 +942,15 @@ def _step_count(device):
     return _STEPS.get(device.index, 0)
 
 
-PREFETCH_PRIORITY = int(os.environ.get("SCN_PREFETCH_PRIORITY", "-1"))  # HIP stream priority of the rule-build side stream (-1 = high)
+# HIP stream priority of the rule-build side stream: the default one (streams of different priorities beside each other have hung the
+# device; a high priority measured no faster step)
+PREFETCH_PRIORITY = 0
 
 
 def prefetch_input(spatialSize, coords, mode, device, wait_for_current_stream=True, normals=None,
                    normal_guide_scale=None):
     """Build the grids and (replaying the previous forward pass's requests) the rulebooks that the next
-    ``InputLayer`` call on exactly this ``coords`` tensor will need, on a high-priority side stream, so that
+    ``InputLayer`` call on exactly this ``coords`` tensor will need, on a side stream, so that
     the build and its data-dependent host synchronisations overlap the current step's queued kernels.  The
     InputLayer call then adopts the result instead of building (it waits on an event, not on the host).
     ``coords`` must not be modified in between.  ``wait_for_current_stream=False`` may be passed when a CUDA
