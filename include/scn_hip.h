@@ -8,7 +8,8 @@
  * reference tree.  Conventions:
  *   - all pointers are DEVICE pointers unless the name ends in `_host`;
  *   - features are contiguous fp32 [rows, planes]; indices are int32 (`Int`,
- *     sparseconvnet/SCN/Metadata/32bits.h:11);
+ *     sparseconvnet/SCN/Metadata/32bits.h:11);  the pointwise operators at the end take a `dtype` besides, and rows
+ *     at a stride where they name one;
  *   - `stream` is a hipStream_t passed as void*; nothing runs on another stream;
  *   - the only entry points that synchronise the stream are those whose
  *     result sizes the next allocation (scn_grid_build, scn_input_rules_max_active,
@@ -450,6 +451,57 @@ int scn_segment_gather(const float *table, const int64_t *seg, const float *scal
                        int S, float *out, void *stream);
 int scn_segment_sqdev(const float *src, const float *mean, const int64_t *seg, int64_t P, int C, int S,
                       float *out, void *stream);
+
+/* ------------------------------------------------- pointwise operators ---
+ * (not in the reference) group norm over ragged samples, dropout, the 1x1 convolution with its epilogue.  Features are
+ * [N, planes] of `dtype`; sums, statistics and products are fp32 or wider whatever it is. */
+#define SCN_F32 0
+#define SCN_BF16 1
+#define SCN_F16 2
+#define SCN_ACT_LEAKY 0 /* z > 0 ? z : leakiness z  (0 = ReLU, 1 = none) */
+#define SCN_ACT_SILU 1  /* z / (1 + exp(-z)) */
+#define SCN_ACT_GELU 2  /* z Phi(z) */
+#define SCN_GROUP_NORM_MAX_PLANES 4096
+
+/* offsets[s], s = 0..samples: first site of sample s (the sites of a grid are in sample order); offsets[samples] = N */
+int scn_sample_offsets(const uint64_t *site_keys, int64_t N, int64_t samples, int64_t *offsets, void *stream);
+
+/* y = act((x - mean) rstd weight + bias), mean and 1 / rstd^2 - eps the mean and variance of the sites of one sample and the
+ * planes / groups planes of one group.  offsets int64 [samples + 1] ascending in 0..N; rows in front of the first sample and
+ * behind the last are neither read nor written.  weight / bias fp32 [planes] or NULL; stats fp32 [samples][groups][2] = (mean,
+ * rstd), zeros for a sample without sites.  x and y contiguous; temp: scn_group_norm_temp_bytes. */
+size_t scn_group_norm_temp_bytes(int64_t N, int planes, int groups, int64_t samples, int dtype, int backward);
+int scn_group_norm_forward(const void *x, void *y, float *stats, const int64_t *offsets, const float *weight,
+                           const float *bias, double eps, int act, double leakiness, int64_t N, int planes, int groups,
+                           int64_t samples, int dtype, void *temp, size_t temp_bytes, void *stream);
+/* d_x of `dtype`; d_weight / d_bias fp32 [planes], assigned (NULL: not wanted) */
+int scn_group_norm_backward(const void *x, const void *d_y, void *d_x, const float *stats, const int64_t *offsets,
+                            const float *weight, const float *bias, float *d_weight, float *d_bias, int act,
+                            double leakiness, int64_t N, int planes, int groups, int64_t samples, int dtype, void *temp,
+                            size_t temp_bytes, void *stream);
+
+/* y[r, c] = word(r, c) >= p 2^32 ? x[r, c] / (1 - p) : 0, 0 <= p < 1.  word(r, c) = word c % 4 of Philox4x32-10 with the key
+ * (low, high half of rng[0]) and the counter (c / 4, r, low, high half of rng[1]); rng int64 [2] = (seed, offset) on the device.
+ * The gradient is the same call on d_y.  x rows at ldx elements, y contiguous. */
+int scn_dropout(const void *x, int64_t ldx, void *y, int64_t N, int planes, int dtype, double p, const int64_t *rng,
+                void *stream);
+/* used = state; state[1] += 1 */
+int scn_rng_take(int64_t *state, int64_t *used, void *stream);
+
+/* y = residual + drop(act(x weight + bias)): weight [n_in, n_out], bias [n_out] or NULL, residual rows at ld_res elements or NULL,
+ * drop as scn_dropout (p 0: none, rng NULL).  factor (NULL: not wanted) [N, n_out] = d y / d (x weight + bias), for the backward
+ * pass.  All of `dtype`; x rows at ldx elements, y and factor contiguous. */
+int scn_linear_forward(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_res,
+                       void *y, void *factor, int64_t N, int n_in, int n_out, int act, double leakiness, double p,
+                       const int64_t *rng, int dtype, void *stream);
+/* d_x = (d_y factor) weight^T; factor NULL: ones.  d_y rows at ld_dy elements */
+int scn_linear_dinput(const void *d_y, int64_t ld_dy, const void *factor, const void *weight, void *d_x, int64_t N, int n_in,
+                      int n_out, int dtype, void *stream);
+/* d_weight = x^T (d_y factor), d_bias = column sums of (d_y factor) (NULL: not wanted), of `dtype`, assigned; partial sums are
+ * added in a fixed order.  temp: scn_linear_dweight_temp_bytes */
+size_t scn_linear_dweight_temp_bytes(int64_t N, int n_in, int n_out);
+int scn_linear_dweight(const void *x, int64_t ldx, const void *d_y, int64_t ld_dy, const void *factor, void *d_weight,
+                       void *d_bias, int64_t N, int n_in, int n_out, int dtype, void *temp, size_t temp_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -369,6 +369,8 @@ class Metadata_3(object):
         self._chain_counts = {}   # spatial size -> N from the grid chain (scn_grid_chain_counts), this batch
         self._occ = None          # (scn_occ_box, buffer) between scn_occ_chain and scn_batch_build_occ
         self._grid_status = []    # (device [N, error flag] of a grid built without read-back, the N it was built for)
+        self.nSamples = None      # largest sample index of the batch + 1, once somebody has needed or found it
+        self._sample_offsets = {} # spatial size -> int64 [nSamples + 1] on the device, see sampleOffsets
 
     def setNormalGuideScale(self, s):
         self.normal_guide_scale = int(s)
@@ -567,6 +569,7 @@ class Metadata_3(object):
             check(lib.scn_occ_bounds(ptr(c), _COORD_DTYPES[c.dtype], c.size(1), P, ptr(scratch), mm, stream()))
             box = _lib.OccBox()
             check(lib.scn_occ_plan(mm, len(sizes), ctypes.byref(box)))
+            self.nSamples = mm[7] + 1  # (max of the sample column)
             if box.bytes > 0 and (occ is True or box.woff[len(sizes)] <= max(1 << 20, OCC_WORDS_PER_ROW * P)):
                 buf = torch.empty(box.bytes, dtype=torch.uint8, device=c.device)
                 check(lib.scn_occ_chain(ptr(c), _COORD_DTYPES[c.dtype], c.size(1), P, ctypes.byref(box), ptr(buf), box.bytes,
@@ -766,6 +769,23 @@ class Metadata_3(object):
     def getSpatialLocations(self, spatialSize):
         """LongTensor [N,4] = (x,y,z,batch) in site order (sparseconvnet/SCN/Metadata/Metadata.cpp:722-749)."""
         return self.grids[_size_key(spatialSize)].coords.cpu().to(torch.int64)
+
+    def sampleOffsets(self, spatialSize):
+        """int64 [samples + 1] on the device: the sites of sample s are rows offsets[s] to offsets[s + 1] of the scale's
+        features.  Made once per batch and scale; the first call of a batch may read the number of samples back."""
+        key = _size_key(spatialSize)
+        offsets = self._sample_offsets.get(key)
+        if offsets is None:
+            g = self.grids[key]
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("occuseg_amd.SCN.sampleOffsets: run the layer once on this batch before capturing it (the number "
+                                   "of samples may have to be read back)")
+            if self.nSamples is None:
+                self.nSamples = (int(g.keys[-1].item()) >> 31) + 1 if g.n else 1
+            offsets = torch.empty(self.nSamples + 1, dtype=torch.int64, device=g.keys.device)
+            check(_lib_().scn_sample_offsets(ptr(g.keys), g.n, self.nSamples, ptr(offsets), stream()))
+            self._sample_offsets[key] = offsets
+        return offsets
 
     # -- rulebooks -----------------------------------------------------------
     def _tile_bases(self, rb, out_col, n_out):
@@ -1858,6 +1878,225 @@ def NetworkInNetwork_accGradParameters(input_features, d_output_features, d_weig
         torch.mm(input_features.t(), d_output_features, out=d_weight)
 
 
+# ------------------------------------------------------- pointwise operators ---
+# (not in the reference) group norm over the samples of a batch, dropout, the 1x1 convolution with its epilogue.  float32,
+# bfloat16 and float16 features; statistics and sums in fp32 or wider.
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # SCN_F32, SCN_BF16, SCN_F16
+ACTIVATIONS = {"leaky_relu": 0, "silu": 1, "gelu": 2}              # SCN_ACT_*
+
+
+def _pointwise(what, x, *others):
+    """refuse what the kernels do not take; returns the dtype code.  ``others``: tensors that must share x's device and dtype
+    (None and empty ones: absent)"""
+    if not torch.is_tensor(x) or x.dim() != 2:
+        raise RuntimeError("occuseg_amd.SCN.%s: features must be a [sites, planes] tensor" % what)
+    if not x.is_cuda:
+        raise RuntimeError("occuseg_amd.SCN.%s: features must live on the GPU -- this backend has no CPU path" % what)
+    code = _DTYPES.get(x.dtype)
+    if code is None:
+        raise RuntimeError("occuseg_amd.SCN.%s: float32, bfloat16 or float16 features, not %s" % (what, x.dtype))
+    for t in others:
+        if t is not None and t.numel() and (t.device != x.device or t.dtype != x.dtype):
+            raise RuntimeError("occuseg_amd.SCN.%s: a %s tensor on %s beside %s features on %s" % (what, t.dtype, t.device, x.dtype,
+                                                                                              x.device))
+    return code
+
+
+def _activation(what, activation):
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError("occuseg_amd.SCN.%s: activation %r is none of %s" % (what, activation, ", ".join(sorted(ACTIVATIONS))))
+    return code
+
+
+def _rows(t):
+    """the tensor and its row stride in elements: rows of consecutive planes are read where they are (a column slice of a wider
+    tensor), anything else is copied"""
+    if t.is_contiguous():
+        return t, t.size(1)
+    if t.stride(1) == 1 and t.stride(0) >= t.size(1):
+        return t, t.stride(0)
+    return t.contiguous(), t.size(1)
+
+
+_NO_DEVICE_CHANGE = contextlib.nullcontext()
+
+
+def _on(t):
+    """launches go to the current stream of the tensor's device, whichever device is current"""
+    return _NO_DEVICE_CHANGE if t.device.index == _lib._cur_device() else torch.cuda.device(t.device)
+
+
+def _opt(t):
+    return t if t is not None and t.numel() else None
+
+
+def _rng(what, rng, x):
+    if not (torch.is_tensor(rng) and rng.dtype == torch.int64 and rng.numel() == 2 and rng.is_contiguous() and rng.device == x.device):
+        raise RuntimeError("occuseg_amd.SCN.%s: rng must be an int64 tensor (seed, offset) on the features' device" % what)
+    return rng
+
+
+def _drop_p(what, p):
+    p = float(p)
+    if not 0.0 <= p < 1.0:
+        raise ValueError("occuseg_amd.SCN.%s: the dropout probability must be in [0, 1), not %r" % (what, p))
+    return p
+
+
+def _group_norm_args(what, features, offsets, weight, bias, groups, activation):
+    code = _pointwise(what, features)
+    N, C = features.shape
+    groups = int(groups)
+    if groups < 1 or C < 1 or C % groups:
+        raise RuntimeError("occuseg_amd.SCN.%s: %d planes do not divide into %d groups" % (what, C, groups))
+    if not (torch.is_tensor(offsets) and offsets.dtype == torch.int64 and offsets.dim() == 1 and offsets.numel() >= 2
+            and offsets.is_contiguous() and offsets.device == features.device):
+        raise RuntimeError("occuseg_amd.SCN.%s: offsets must be an int64 tensor [samples + 1] on the features' device" % what)
+    for t in (_opt(weight), _opt(bias)):
+        if t is not None and not (t.dtype == torch.float32 and t.numel() == C and t.is_contiguous() and t.device == features.device):
+            raise RuntimeError("occuseg_amd.SCN.%s: weight and bias must be float32 [%d] on the features' device" % (what, C))
+    return code, N, C, groups, offsets.numel() - 1, _activation(what, activation)
+
+
+def GroupNormalization_updateOutput(input_features, output_features, stats, offsets, weight, bias, eps, groups, activation, leakiness):
+    """Normalise each of ``groups`` groups of consecutive planes over the sites of each sample, scale, shift, activate.  ``offsets``
+    int64 [samples + 1]: see Metadata_3.sampleOffsets; rows outside of 0..offsets[-1] are left as ``resize_`` leaves them.
+    ``stats`` receives (mean, 1 / sqrt(var + eps)) as float32 [samples, groups, 2], which the backward pass takes."""
+    what = "GroupNormalization_updateOutput"
+    code, N, C, groups, S, act = _group_norm_args(what, input_features, offsets, weight, bias, groups, activation)
+    x = input_features.contiguous()
+    lib = _lib_()
+    with _on(x):
+        output_features.resize_(N, C)
+        stats.resize_(S, groups, 2)
+        tb = lib.scn_group_norm_temp_bytes(N, C, groups, S, code, 0)
+        temp = torch.empty(tb, dtype=torch.uint8, device=x.device)
+        ev = _prof_begin("bn")
+        check(lib.scn_group_norm_forward(ptr(x), ptr(output_features), ptr(stats), ptr(offsets), ptr(_opt(weight)), ptr(_opt(bias)),
+                                         float(eps), act, float(leakiness), N, C, groups, S, code, ptr(temp), tb, stream()))
+        _prof_end(ev, "gn_fwd", 0.0, 3.0 * N * C * x.element_size(), (N, C, groups))
+
+
+def GroupNormalization_backward(input_features, d_input_features, d_output_features, stats, offsets, weight, bias, d_weight, d_bias,
+                                groups, activation, leakiness):
+    """d_weight / d_bias (float32 [planes], empty: not wanted) are assigned"""
+    what = "GroupNormalization_backward"
+    code, N, C, groups, S, act = _group_norm_args(what, input_features, offsets, weight, bias, groups, activation)
+    _pointwise(what, d_output_features, input_features)
+    if d_output_features.shape != input_features.shape or stats.numel() != 2 * S * groups or stats.dtype != torch.float32:
+        raise RuntimeError("occuseg_amd.SCN.%s: shapes" % what)
+    x, dy = input_features.contiguous(), d_output_features.contiguous()
+    lib = _lib_()
+    with _on(x):
+        d_input_features.resize_(N, C)
+        tb = lib.scn_group_norm_temp_bytes(N, C, groups, S, code, 1)
+        temp = torch.empty(tb, dtype=torch.uint8, device=x.device)
+        ev = _prof_begin("bn")
+        check(lib.scn_group_norm_backward(ptr(x), ptr(dy), ptr(d_input_features), ptr(stats), ptr(offsets), ptr(_opt(weight)),
+                                          ptr(_opt(bias)), ptr(_opt(d_weight)), ptr(_opt(d_bias)), act, float(leakiness), N, C, groups,
+                                          S, code, ptr(temp), tb, stream()))
+        _prof_end(ev, "gn_bwd", 0.0, 5.0 * N * C * x.element_size(), (N, C, groups))
+
+
+def Dropout_updateOutput(input_features, output_features, p, rng):
+    """output = input / (1 - p) where the site's random word is at least p 2^32, else 0.  The words are a function of (seed, offset)
+    in ``rng``, the site and the plane (Philox4x32-10): the same ``rng`` gives the same mask, nothing is stored."""
+    what = "Dropout_updateOutput"
+    code, p = _pointwise(what, input_features), _drop_p(what, p)
+    rng = _rng(what, rng, input_features)
+    x, ld = _rows(input_features)
+    N, C = x.shape
+    with _on(x):
+        output_features.resize_(N, C)
+        if C:
+            check(_lib_().scn_dropout(ptr(x), ld, ptr(output_features), N, C, code, p, ptr(rng), stream()))
+
+
+def Dropout_updateGradInput(d_input_features, d_output_features, p, rng):
+    """the same mask, made again from the forward pass's ``rng``"""
+    Dropout_updateOutput(d_output_features, d_input_features, p, rng)
+
+
+def rng_take(state):
+    """(seed, offset) of ``state`` as a new tensor; the state moves on by one.  On the device: a captured graph draws anew at every
+    replay."""
+    if not state.is_cuda:
+        raise RuntimeError("occuseg_amd.SCN.rng_take: the state must live on the GPU")
+    used = torch.empty(2, dtype=torch.int64, device=state.device)
+    with _on(state):
+        check(_lib_().scn_rng_take(ptr(_rng("rng_take", state, state)), ptr(used), stream()))
+    return used
+
+
+def _linear_args(what, features, weight, bias):
+    code = _pointwise(what, features, weight, bias)
+    if weight.dim() != 2 or weight.size(0) < 1 or weight.size(1) < 1 or features.size(1) != weight.size(0):
+        raise RuntimeError("occuseg_amd.SCN.%s: features %s and weight %s" % (what, tuple(features.shape), tuple(weight.shape)))
+    if _opt(bias) is not None and bias.numel() != weight.size(1):
+        raise RuntimeError("occuseg_amd.SCN.%s: weight %s and bias %s" % (what, tuple(weight.shape), tuple(bias.shape)))
+    return code, features.size(0), weight.size(0), weight.size(1)
+
+
+def FusedNetworkInNetwork_updateOutput(input_features, output_features, weight, bias, residual, activation, leakiness, p, rng,
+                                       factor=None):
+    """output = residual + dropout(act(input @ weight + bias)) in one kernel.  ``residual`` None: none; ``p`` 0: no dropout, ``rng``
+    None.  ``factor`` (an empty tensor, training) receives d output / d (input @ weight + bias) for the backward pass."""
+    what = "FusedNetworkInNetwork_updateOutput"
+    code, N, Ci, Co = _linear_args(what, input_features, weight, bias)
+    act, p = _activation(what, activation), _drop_p(what, p)
+    rng = _rng(what, rng, input_features) if p > 0 else None
+    x, ld = _rows(input_features)
+    bias = bias.contiguous() if _opt(bias) is not None else None
+    res, ld_res = None, 0
+    if residual is not None:
+        _pointwise(what, residual, x)
+        if tuple(residual.shape) != (N, Co):
+            raise RuntimeError("occuseg_amd.SCN.%s: residual %s for an output of %s" % (what, tuple(residual.shape), (N, Co)))
+        res, ld_res = _rows(residual)
+    with _on(x):
+        output_features.resize_(N, Co)
+        if factor is not None:
+            factor.resize_(N, Co)
+        ev = _prof_begin()
+        check(_lib_().scn_linear_forward(ptr(x), ld, ptr(weight.contiguous()), ptr(bias), ptr(res), ld_res, ptr(output_features),
+                                         ptr(factor), N, Ci, Co, act, float(leakiness), p, ptr(rng), code, stream()))
+        _prof_end(ev, "linear_fwd", 2.0 * N * Ci * Co,
+                  float(x.element_size()) * (N * (Ci + Co * (1 + (res is not None) + (factor is not None))) + Ci * Co), (N, Ci, Co))
+    return float(N) * Ci * Co
+
+
+def FusedNetworkInNetwork_backward(input_features, d_input_features, d_output_features, weight, d_weight, d_bias, factor=None):
+    """d_input (None: not wanted), d_weight and d_bias (None: not wanted) are assigned; ``factor`` as the forward pass left it, None:
+    the pass had neither activation nor dropout.  The residual's gradient is d_output itself."""
+    what = "FusedNetworkInNetwork_backward"
+    code, N, Ci, Co = _linear_args(what, input_features, weight, None)
+    _pointwise(what, d_output_features, input_features, factor)
+    if tuple(d_output_features.shape) != (N, Co) or (factor is not None and tuple(factor.shape) != (N, Co)):
+        raise RuntimeError("occuseg_amd.SCN.%s: shapes" % what)
+    x, ldx = _rows(input_features)
+    dy, ld_dy = _rows(d_output_features)
+    lib = _lib_()
+    with _on(x):
+        es = float(x.element_size())
+        if d_input_features is not None:
+            d_input_features.resize_(N, Ci)
+            ev = _prof_begin()
+            check(lib.scn_linear_dinput(ptr(dy), ld_dy, ptr(factor), ptr(weight.contiguous()), ptr(d_input_features), N, Ci, Co, code,
+                                        stream()))
+            _prof_end(ev, "linear_dx", 2.0 * N * Ci * Co, es * (N * (Ci + Co * (1 + (factor is not None))) + Ci * Co), (N, Ci, Co))
+        if d_weight is not None:
+            d_weight.resize_(Ci, Co)
+            if d_bias is not None:
+                d_bias.resize_(Co)
+            tb = lib.scn_linear_dweight_temp_bytes(N, Ci, Co)
+            temp = torch.empty(tb, dtype=torch.uint8, device=x.device)
+            ev = _prof_begin()
+            check(lib.scn_linear_dweight(ptr(x), ldx, ptr(dy), ld_dy, ptr(factor), ptr(d_weight), ptr(d_bias), N, Ci, Co, code,
+                                         ptr(temp), tb, stream()))
+            _prof_end(ev, "linear_dw", 2.0 * N * Ci * Co, es * (N * (Ci + Co * (1 + (factor is not None))) + Ci * Co), (N, Ci, Co))
+
+
 def _not_in_scope(name):
     def f(*a, **k):
         raise NotImplementedError("sparseconvnet.SCN.%s is outside the hot path this backend provides "
@@ -1909,7 +2148,8 @@ _TRACED = ("InputLayer_updateOutput", "InputLayer_updateGradInput", "OutputLayer
            "SubmanifoldConvolution_updateOutput", "SubmanifoldConvolution_backward", "Convolution_updateOutput",
            "Convolution_backward", "Deconvolution_updateOutput", "Deconvolution_backward", "BatchNormalization_updateOutput",
            "BatchNormalization_backward", "NetworkInNetwork_updateOutput", "NetworkInNetwork_updateGradInput",
-           "NetworkInNetwork_backward")
+           "NetworkInNetwork_backward", "GroupNormalization_updateOutput", "GroupNormalization_backward", "Dropout_updateOutput",
+           "FusedNetworkInNetwork_updateOutput", "FusedNetworkInNetwork_backward")
 
 
 def _traced(name, fn):

@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libscn_hip.so")
 LIB_TUNING = os.path.join(HERE, "libscn_hip_tuning.so")
-SOURCES = ["scn_rules.hip", "scn_dense.hip", "scn_conv.hip", "scn_aux.hip"]
+SOURCES = ["scn_rules.hip", "scn_dense.hip", "scn_conv.hip", "scn_aux.hip", "scn_groupnorm.hip", "scn_linear.hip"]
 TUNING_ONLY = ["scn_peaks.hip"]  # measured-peak microbenchmarks: tools/peaks.py, bench.py's roofline
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics"]
 # hipcc makes v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32 of ordinary float code by itself, and some of their forms have given wrong
@@ -29,7 +29,7 @@ def _stale(target, deps):
 
 def build(force=False, verbose=True, tuning=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    headers = [os.path.join(CSRC, "scn_common.h"), os.path.join(HERE, "..", "include", "scn_hip.h"),
+    headers = [os.path.join(CSRC, "scn_common.h"), os.path.join(CSRC, "scn_pointwise.h"), os.path.join(HERE, "..", "include", "scn_hip.h"),
                os.path.join(CSRC, "tile4_loop_asm.inc"), os.path.join(CSRC, "tile4_loop_asm_tuning.inc")]
     # k_conv_tile4's pass loop in assembly is GENERATED (tools/gen_tile4_loop.py, which also proves on its own instruction list
     # that no instruction touches a register with a load in flight): the committed file must be what the generator writes

@@ -1,0 +1,496 @@
+// Group norm over ragged samples with its activation, channels last (gfx950); the sample offsets it runs over.
+//
+//   y = act((x - mean_sg) rstd_sg w_c + b_c),   statistics over the n_s sites of sample s x the C / G planes of group g
+//   dz = dy act'(z), xh = (x - mean) rstd, dn = dz w:
+//   dx = rstd (dn - <dn> - xh <dn xh>),  db_c = sum dz,  dw_c = sum dz xh      (<> over the same n_s C / G values)
+//
+// HBM bound: forward reads x twice and writes y, backward reads x and dy twice and writes dx; a sample's values are needed before
+// its statistics are known, and 154 MB (600k sites x 64 planes) do not stay on the chip.
+//
+// Three launches a direction: sums per CHUNK of rows, a join of the chunks in fp64 in a fixed order, the apply pass.  A chunk is
+// 2^shift rows of one sample: chunk b belongs to the last sample s with (offsets[s] >> shift) + s <= b, which needs no table, no
+// read-back of the lengths, and at most (N >> shift) + samples workgroups.  The rows of a chunk are one contiguous span, walked in
+// 16-byte vectors whatever C is: the vectors step through the span by a multiple of lcm(C, vector), so every thread keeps the same
+// planes, and their constants, for the whole chunk.
+#include "scn_pointwise.h"
+
+#include <type_traits>
+
+namespace scn {
+
+struct GnArgs {
+  const int64_t *offsets;
+  int64_t N;
+  int S, C, G, cpg;
+  int shift;   // rows per chunk = 1 << shift
+  int period;  // vectors per lcm(C, V) elements; a thread steps by a multiple of it
+  int step;    // ... this many vectors (a multiple of `period`; of at most 256 vectors if that is possible)
+  float leak;
+};
+
+// the sample and the rows of chunk b; false: an empty chunk.  Every wave finds it by itself, 64 samples a step.
+__device__ __forceinline__ bool gn_chunk(const GnArgs &a, int64_t b, int &s, int64_t &r0, int64_t &r1) {
+  int below = 0;
+  for (int base = 0; base < a.S; base += 64) {
+    const int i = base + lane_id();
+    const bool in = i < a.S && (a.offsets[min(i, a.S - 1)] >> a.shift) + i <= b;
+    const int n = __popcll(__ballot(in));
+    below += n;
+    if (n < 64) break;
+  }
+  if (below == 0) return false;
+  s = below - 1;
+  const int64_t start = max(a.offsets[s], (int64_t)0), end = min(a.offsets[s + 1], a.N);
+  r0 = start + ((b - ((start >> a.shift) + s)) << a.shift);
+  r1 = min(r0 + ((int64_t)1 << a.shift), end);
+  return r0 < r1;
+}
+
+// f(i, vector) for the thread's vectors of the span [0, span) of p: vector q, q + step, ...; the span's last vector may be partial,
+// its missing elements are `fill`.
+template <int UNROLL, class T, int V, class F>
+__device__ __forceinline__ void gn_walk(const T *p, int span, int q, int step, F &&f) {
+  int i = q * V;
+  const int d = step * V;
+  for (; i + (UNROLL - 1) * d + V <= span; i += UNROLL * d) {
+    Pack<T, V> v[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) v[u] = load_pack<T, V>(p + i + u * d);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) f(i + u * d, V, v[u]);
+  }
+  for (; i < span; i += d) {
+    Pack<T, V> v;
+    const int n = min(V, span - i);
+    if (n == V) v = load_pack<T, V>(p + i);
+    else
+#pragma unroll
+      for (int j = 0; j < V; ++j) v.v[j] = j < n ? p[i + j] : (T)0.f;
+    f(i, n, v);
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void gn_store(T *p, int n, const Pack<T, V> &v) {
+  if (n == V) store_pack<T, V>(p, v);
+  else
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < n) p[j] = v.v[j];
+}
+
+// ------------------------------------------------------------------ forward ---
+// partial[chunk][group] = (mean, sum of squared deviations).  Every thread sums its planes' deviations from the plane's first value
+// in the chunk: sums of squares of values far from zero would cancel.  The entries are joined by the deviations of their means.
+template <class T, int V>
+__global__ void __launch_bounds__(256) k_gn_stats(const T *x, GnArgs a, float2 *partial) {
+  extern __shared__ float2 ent[];  // [step * V] (mean, squared deviations) per element of a step
+  int s;
+  int64_t r0, r1;
+  if (!gn_chunk(a, blockIdx.x, s, r0, r1)) return;
+  const int span = (int)(r1 - r0) * a.C, E = a.step * V;
+  const T *p = x + r0 * a.C;
+  for (int q = threadIdx.x; q < a.step; q += 256) {
+    float pivot[V], s1[V], s2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      pivot[j] = q * V + j < span ? (float)p[q * V + j] : 0.f;
+      s1[j] = s2[j] = 0.f;
+    }
+    gn_walk<4, T, V>(p, span, q, a.step, [&](int, int n, const Pack<T, V> &v) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = j < n ? (float)v.v[j] - pivot[j] : 0.f;
+        s1[j] += d;
+        s2[j] = fmaf(d, d, s2[j]);
+      }
+    });
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int e = q * V + j;
+      const float n = (float)((span - e + E - 1) / E);
+      const float m = e < span ? s1[j] / n : 0.f;
+      ent[e] = make_float2(pivot[j] + m, e < span ? fmaxf(s2[j] - s1[j] * m, 0.f) : 0.f);
+    }
+  }
+  __syncthreads();
+  // tpg threads (a power of two, within a wave) per group
+  int tpg = 64;
+  while (tpg > 1 && tpg * a.G > 256) tpg >>= 1;
+  const int sub = threadIdx.x & (tpg - 1), entries = E / a.C * a.cpg;
+  for (int g0 = 0; g0 < a.G; g0 += 256 / tpg) {
+    const int g = g0 + threadIdx.x / tpg;
+    const bool on = g < a.G;
+    float pv = 0.f, sum = 0.f, sq = 0.f, mean = 0.f;
+    if (on) {
+      pv = ent[g * a.cpg].x;  // (row 0 is there)
+      for (int i = sub; i < entries; i += tpg) {
+        const int e = i / a.cpg * a.C + g * a.cpg + i % a.cpg;
+        if (e < span) sum += (float)((span - e + E - 1) / E) * (ent[e].x - pv);
+      }
+    }
+    for (int o = 1; o < tpg; o <<= 1) sum += __shfl_xor(sum, o);
+    if (on) {
+      mean = pv + sum / (float)((int)(r1 - r0) * a.cpg);
+      for (int i = sub; i < entries; i += tpg) {
+        const int e = i / a.cpg * a.C + g * a.cpg + i % a.cpg;
+        if (e < span) {
+          const float d = ent[e].x - mean;
+          sq += fmaf((float)((span - e + E - 1) / E) * d, d, ent[e].y);
+        }
+      }
+    }
+    for (int o = 1; o < tpg; o <<= 1) sq += __shfl_xor(sq, o);
+    if (on && sub == 0) partial[(int64_t)blockIdx.x * a.G + g] = make_float2(mean, sq);
+  }
+}
+
+// stats[s][g] = (mean, rstd): the chunks' means and deviations joined in fp64, in chunk order.  Workgroup (y, s): up to 1024 groups
+// of one sample, every group by 1024 / groups threads.
+__global__ void __launch_bounds__(1024) k_gn_join(const float2 *partial, GnArgs a, double eps, float2 *stats) {
+  __shared__ double red[2][1024];
+  const int s = blockIdx.x, g0 = blockIdx.y * 1024, gb = min(a.G - g0, 1024), slots = 1024 / gb;
+  const int gl = threadIdx.x % gb, slot = threadIdx.x / gb;
+  const int64_t start = max(a.offsets[s], (int64_t)0), end = min(a.offsets[s + 1], a.N), rows = end - start;
+  const int64_t b0 = (start >> a.shift) + s;
+  const int chunks = rows > 0 ? (int)((rows + ((int64_t)1 << a.shift) - 1) >> a.shift) : 0;
+  double s1 = 0, s2 = 0;
+  if (slot < slots)
+#pragma unroll 4
+    for (int c = slot; c < chunks; c += slots) {
+      const float2 v = partial[(b0 + c) * a.G + g0 + gl];
+      const double n = (double)min(rows - ((int64_t)c << a.shift), (int64_t)1 << a.shift) * a.cpg, m = v.x;
+      s1 += n * m;
+      s2 += (double)v.y + n * m * m;
+    }
+  red[0][threadIdx.x] = s1;
+  red[1][threadIdx.x] = s2;
+  __syncthreads();
+  if (slot != 0) return;
+  for (int k = 1; k < slots; ++k) {
+    s1 += red[0][k * gb + gl];
+    s2 += red[1][k * gb + gl];
+  }
+  float2 out = make_float2(0.f, 0.f);
+  if (chunks > 0) {
+    const double n = (double)rows * a.cpg, m = s1 / n, var = fmax(s2 / n - m * m, 0.0);
+    out = make_float2((float)m, (float)(1.0 / sqrt(var + eps)));
+  }
+  // (NaN in the sample: fmax drops it; the mean has it)
+  stats[(int64_t)s * a.G + g0 + gl] = out;
+}
+
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(256)
+    k_gn_apply(const T *x, T *y, GnArgs a, const float2 *stats, const float *weight, const float *bias) {
+  int s;
+  int64_t r0, r1;
+  if (!gn_chunk(a, blockIdx.x, s, r0, r1)) return;
+  const int span = (int)(r1 - r0) * a.C;
+  const T *p = x + r0 * a.C;
+  T *o = y + r0 * a.C;
+  constexpr bool EXACT = sizeof(T) == 4;
+  for (int q = threadIdx.x; q < a.step; q += 256) {
+    float mean[V], w[V], b[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (q * V + j) % a.C;
+      const float2 st = stats[(int64_t)s * a.G + c / a.cpg];
+      mean[j] = st.x;
+      w[j] = st.y * (weight ? weight[c] : 1.f);
+      b[j] = bias ? bias[c] : 0.f;
+    }
+    gn_walk<4, T, V>(p, span, q, a.step, [&](int i, int n, const Pack<T, V> &v) {
+      Pack<T, V> r;
+#pragma unroll
+      for (int j = 0; j < V; ++j) r.v[j] = (T)act_value<ACT, EXACT>(fmaf((float)v.v[j] - mean[j], w[j], b[j]), a.leak);
+      gn_store<T, V>(o + i, n, r);
+    });
+  }
+}
+
+// ----------------------------------------------------------------- backward ---
+// partial[chunk][plane] = (sum dz, sum dz xh)
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(256)
+    k_gn_bwd_sums(const T *x, const T *dy, GnArgs a, const float2 *stats, const float *weight, const float *bias, float2 *partial) {
+  extern __shared__ float2 ent[];
+  int s;
+  int64_t r0, r1;
+  if (!gn_chunk(a, blockIdx.x, s, r0, r1)) return;
+  const int span = (int)(r1 - r0) * a.C, E = a.step * V;
+  const T *p = x + r0 * a.C, *g = dy + r0 * a.C;
+  constexpr bool EXACT = sizeof(T) == 4;
+  for (int q = threadIdx.x; q < a.step; q += 256) {
+    float mean[V], rstd[V], w[V], b[V], s1[V], s2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (q * V + j) % a.C;
+      const float2 st = stats[(int64_t)s * a.G + c / a.cpg];
+      mean[j] = st.x;
+      rstd[j] = st.y;
+      w[j] = st.y * (weight ? weight[c] : 1.f);
+      b[j] = bias ? bias[c] : 0.f;
+      s1[j] = s2[j] = 0.f;
+    }
+    gn_walk<4, T, V>(p, span, q, a.step, [&](int i, int n, const Pack<T, V> &v) {
+      Pack<T, V> d;
+      if (n == V) d = load_pack<T, V>(g + i);
+      else
+#pragma unroll
+        for (int j = 0; j < V; ++j) d.v[j] = j < n ? g[i + j] : (T)0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float c = (float)v.v[j] - mean[j];
+        const float dz = j < n ? (float)d.v[j] * act_slope<ACT, EXACT>(fmaf(c, w[j], b[j]), a.leak) : 0.f;
+        s1[j] += dz;
+        s2[j] = fmaf(dz, c * rstd[j], s2[j]);
+      }
+    });
+#pragma unroll
+    for (int j = 0; j < V; ++j) ent[q * V + j] = make_float2(s1[j], s2[j]);
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.C; c += 256) {
+    float2 t = ent[c];
+    for (int e = c + a.C; e < E; e += a.C) {
+      t.x += ent[e].x;
+      t.y += ent[e].y;
+    }
+    partial[(int64_t)blockIdx.x * a.C + c] = t;
+  }
+}
+
+// sums[s][plane]: the chunks of one sample, fp64, in chunk order; 16 planes x 64 slots a workgroup
+__global__ void __launch_bounds__(1024) k_gn_bwd_join(const float2 *partial, GnArgs a, float2 *sums) {
+  __shared__ double red[2][64][17];
+  const int s = blockIdx.x, cl = threadIdx.x & 15, slot = threadIdx.x >> 4, c = blockIdx.y * 16 + cl;
+  const int64_t start = max(a.offsets[s], (int64_t)0), end = min(a.offsets[s + 1], a.N), rows = end - start;
+  const int64_t b0 = (start >> a.shift) + s;
+  const int chunks = rows > 0 ? (int)((rows + ((int64_t)1 << a.shift) - 1) >> a.shift) : 0;
+  double s1 = 0, s2 = 0;
+  if (c < a.C)
+#pragma unroll 4
+    for (int k = slot; k < chunks; k += 64) {
+      const float2 v = partial[(b0 + k) * a.C + c];
+      s1 += v.x;
+      s2 += v.y;
+    }
+  red[0][slot][cl] = s1;
+  red[1][slot][cl] = s2;
+  __syncthreads();
+  if (slot != 0 || c >= a.C) return;
+  for (int k = 1; k < 64; ++k) {
+    s1 += red[0][k][cl];
+    s2 += red[1][k][cl];
+  }
+  sums[(int64_t)s * a.C + c] = make_float2((float)s1, (float)s2);
+}
+
+// dx; the workgroups behind the chunks add the planes' sums over the samples (d_weight, d_bias)
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(256)
+    k_gn_bwd_apply(const T *x, const T *dy, T *dx, GnArgs a, const float2 *stats, const float *weight, const float *bias,
+                   const float2 *sums, float *d_weight, float *d_bias, int chunk_blocks) {
+  extern __shared__ float2 grp[];  // [G] (<dn>, <dn xh>)
+  if ((int)blockIdx.x >= chunk_blocks) {
+    const int c = ((int)blockIdx.x - chunk_blocks) * 256 + threadIdx.x;
+    if (c >= a.C) return;
+    double s1 = 0, s2 = 0;
+    for (int s = 0; s < a.S; ++s) {
+      const float2 v = sums[(int64_t)s * a.C + c];
+      s1 += v.x;
+      s2 += v.y;
+    }
+    if (d_bias) d_bias[c] = (float)s1;
+    if (d_weight) d_weight[c] = (float)s2;
+    return;
+  }
+  int s;
+  int64_t r0, r1;
+  if (!gn_chunk(a, blockIdx.x, s, r0, r1)) return;
+  const int64_t rows = min(a.offsets[s + 1], a.N) - max(a.offsets[s], (int64_t)0);
+  for (int g = threadIdx.x; g < a.G; g += 256) {
+    float m1 = 0.f, m2 = 0.f;
+    for (int c = g * a.cpg; c < (g + 1) * a.cpg; ++c) {
+      const float2 v = sums[(int64_t)s * a.C + c];
+      const float w = weight ? weight[c] : 1.f;
+      m1 = fmaf(w, v.x, m1);
+      m2 = fmaf(w, v.y, m2);
+    }
+    const float n = (float)rows * (float)a.cpg;
+    grp[g] = make_float2(m1 / n, m2 / n);
+  }
+  __syncthreads();
+  const int span = (int)(r1 - r0) * a.C;
+  const T *p = x + r0 * a.C, *g = dy + r0 * a.C;
+  T *o = dx + r0 * a.C;
+  constexpr bool EXACT = sizeof(T) == 4;
+  for (int q = threadIdx.x; q < a.step; q += 256) {
+    float mean[V], rstd[V], w[V], b[V], m1[V], m2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (q * V + j) % a.C, gi = c / a.cpg;
+      const float2 st = stats[(int64_t)s * a.G + gi];
+      mean[j] = st.x;
+      rstd[j] = st.y;
+      w[j] = st.y * (weight ? weight[c] : 1.f);
+      b[j] = bias ? bias[c] : 0.f;
+      m1[j] = grp[gi].x * st.y;
+      m2[j] = grp[gi].y * st.y * st.y;
+    }
+    gn_walk<4, T, V>(p, span, q, a.step, [&](int i, int n, const Pack<T, V> &v) {
+      Pack<T, V> d, r;
+      if (n == V) d = load_pack<T, V>(g + i);
+      else
+#pragma unroll
+        for (int j = 0; j < V; ++j) d.v[j] = j < n ? g[i + j] : (T)0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float c = (float)v.v[j] - mean[j];
+        const float dz = (float)d.v[j] * act_slope<ACT, EXACT>(fmaf(c, w[j], b[j]), a.leak);
+        r.v[j] = (T)(fmaf(dz, w[j], -m1[j]) - c * m2[j]);
+      }
+      gn_store<T, V>(o + i, n, r);
+    });
+  }
+}
+
+// ------------------------------------------------------------ sample offsets ---
+// offsets[s] = first site whose key is at or behind sample s's first key: the keys ascend
+__global__ void k_sample_offsets(const uint64_t *keys, int64_t N, int64_t S, int64_t *offsets) {
+  for (int64_t s = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; s <= S; s += (int64_t)gridDim.x * blockDim.x) {
+    int64_t lo = 0, hi = N;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if ((int64_t)(keys[mid] >> 31) < s) lo = mid + 1; else hi = mid;
+    }
+    offsets[s] = s == S ? N : lo;
+  }
+}
+
+// ---------------------------------------------------------------------- host ---
+static int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+// 16-byte vectors if their period fits a workgroup, single elements else (an odd plane count above 256)
+static bool gn_wide(int C, int V) { return C / gcd(C, V) <= 256 || C % V == 0; }
+
+static GnArgs gn_args(const int64_t *offsets, int64_t N, int C, int G, int64_t S, int dtype, int V, double leak) {
+  GnArgs a;
+  a.offsets = offsets;
+  a.N = N;
+  a.S = (int)S;
+  a.C = C;
+  a.G = G;
+  a.cpg = C / G;
+  a.leak = (float)leak;
+  a.period = C / gcd(C, V);
+  a.step = a.period <= 256 ? 256 / a.period * a.period : a.period;
+  // about 1500 chunks of a large tensor, none below 16 KB: the partial sums stay small against the rows they come from
+  const int64_t row = (int64_t)C * (dtype == SCN_F32 ? 4 : 2);
+  int64_t bytes = N * row / 1024;
+  bytes = bytes < 16384 ? 16384 : bytes > (1 << 20) ? 1 << 20 : bytes;
+  a.shift = 0;
+  while (a.shift < 20 && (row << (a.shift + 1)) <= bytes) ++a.shift;
+  return a;
+}
+static int64_t gn_chunks(const GnArgs &a) { return (a.N >> a.shift) + a.S; }
+
+template <class T, int V>
+static int gn_forward(const void *x, void *y, float *stats, GnArgs a, const float *weight, const float *bias, double eps, int act,
+                      void *temp, hipStream_t st) {
+  const unsigned chunks = (unsigned)gn_chunks(a);
+  float2 *partial = (float2 *)temp;
+  k_gn_stats<T, V><<<chunks, 256, sizeof(float2) * a.step * V, st>>>((const T *)x, a, partial);
+  SCN_CHECK_LAUNCH();
+  k_gn_join<<<dim3(a.S, (a.G + 1023) / 1024), 1024, 0, st>>>(partial, a, eps, (float2 *)stats);
+  SCN_CHECK_LAUNCH();
+  auto apply = act == SCN_ACT_SILU ? k_gn_apply<T, V, SCN_ACT_SILU>
+               : act == SCN_ACT_GELU ? k_gn_apply<T, V, SCN_ACT_GELU> : k_gn_apply<T, V, SCN_ACT_LEAKY>;
+  apply<<<chunks, 256, 0, st>>>((const T *)x, (T *)y, a, (const float2 *)stats, weight, bias);
+  SCN_CHECK_LAUNCH();
+  return 0;
+}
+
+template <class T, int V>
+static int gn_backward(const void *x, const void *dy, void *dx, const float *stats, GnArgs a, const float *weight, const float *bias,
+                       float *d_weight, float *d_bias, int act, void *temp, hipStream_t st) {
+  const unsigned chunks = (unsigned)gn_chunks(a);
+  float2 *partial = (float2 *)temp, *sums = partial + (int64_t)chunks * a.C;
+  auto k1 = act == SCN_ACT_SILU ? k_gn_bwd_sums<T, V, SCN_ACT_SILU>
+            : act == SCN_ACT_GELU ? k_gn_bwd_sums<T, V, SCN_ACT_GELU> : k_gn_bwd_sums<T, V, SCN_ACT_LEAKY>;
+  k1<<<chunks, 256, sizeof(float2) * a.step * V, st>>>((const T *)x, (const T *)dy, a, (const float2 *)stats, weight, bias, partial);
+  SCN_CHECK_LAUNCH();
+  k_gn_bwd_join<<<dim3(a.S, (a.C + 15) / 16), 1024, 0, st>>>(partial, a, sums);
+  SCN_CHECK_LAUNCH();
+  auto k2 = act == SCN_ACT_SILU ? k_gn_bwd_apply<T, V, SCN_ACT_SILU>
+            : act == SCN_ACT_GELU ? k_gn_bwd_apply<T, V, SCN_ACT_GELU> : k_gn_bwd_apply<T, V, SCN_ACT_LEAKY>;
+  k2<<<chunks + (a.C + 255) / 256, 256, sizeof(float2) * a.G, st>>>((const T *)x, (const T *)dy, (T *)dx, a, (const float2 *)stats,
+                                                                  weight, bias, sums, d_weight, d_bias, (int)chunks);
+  SCN_CHECK_LAUNCH();
+  return 0;
+}
+
+static int gn_check(int64_t N, int C, int G, int64_t S, int dtype, int act) {
+  SCN_REQUIRE(dtype == SCN_F32 || dtype == SCN_BF16 || dtype == SCN_F16, "group norm: dtype");
+  SCN_REQUIRE(act == SCN_ACT_LEAKY || act == SCN_ACT_SILU || act == SCN_ACT_GELU, "group norm: activation");
+  SCN_REQUIRE(C >= 1 && C <= SCN_GROUP_NORM_MAX_PLANES, "group norm: 1 to 4096 planes");
+  SCN_REQUIRE(G >= 1 && C % G == 0, "group norm: the planes must divide into the groups");
+  SCN_REQUIRE(S >= 1 && S <= 65535 && N >= 0 && N < ((int64_t)1 << 31), "group norm: 1 to 65535 samples, fewer than 2^31 sites");
+  return 0;
+}
+
+template <class F>
+static int gn_dispatch(int dtype, int C, F &&f) {
+  const bool wide = gn_wide(C, dtype == SCN_F32 ? 4 : 8);
+  if (dtype == SCN_F32) return wide ? f((float)0, std::integral_constant<int, 4>()) : f((float)0, std::integral_constant<int, 1>());
+  if (dtype == SCN_BF16) return wide ? f((__bf16)0, std::integral_constant<int, 8>()) : f((__bf16)0, std::integral_constant<int, 1>());
+  return wide ? f((_Float16)0, std::integral_constant<int, 8>()) : f((_Float16)0, std::integral_constant<int, 1>());
+}
+
+}  // namespace scn
+
+using namespace scn;
+
+extern "C" {
+
+int scn_sample_offsets(const uint64_t *site_keys, int64_t N, int64_t samples, int64_t *offsets, void *stream) {
+  SCN_REQUIRE(N >= 0 && samples >= 1 && samples < ((int64_t)1 << 31) && offsets, "sample offsets: arguments");
+  k_sample_offsets<<<(unsigned)((samples + 256) / 256), 256, 0, as_stream(stream)>>>(site_keys, N, samples, offsets);
+  SCN_CHECK_LAUNCH();
+  return 0;
+}
+
+size_t scn_group_norm_temp_bytes(int64_t N, int planes, int groups, int64_t samples, int dtype, int backward) {
+  if (gn_check(N, planes, groups, samples, dtype, 0)) return 0;
+  const GnArgs a = gn_args(nullptr, N, planes, groups, samples, dtype, 1, 0);
+  return sizeof(float2) * (size_t)(backward ? (gn_chunks(a) + samples) * planes : gn_chunks(a) * groups);
+}
+
+int scn_group_norm_forward(const void *x, void *y, float *stats, const int64_t *offsets, const float *weight, const float *bias,
+                           double eps, int act, double leakiness, int64_t N, int planes, int groups, int64_t samples, int dtype,
+                           void *temp, size_t temp_bytes, void *stream) {
+  if (int e = gn_check(N, planes, groups, samples, dtype, act)) return e;
+  SCN_REQUIRE(stats && offsets && (N == 0 || (x && y)), "group norm: pointers");
+  SCN_REQUIRE(temp && temp_bytes >= scn_group_norm_temp_bytes(N, planes, groups, samples, dtype, 0), "group norm: workspace");
+  return gn_dispatch(dtype, planes, [&](auto t, auto v) {
+    constexpr int V = decltype(v)::value;
+    return gn_forward<decltype(t), V>(x, y, stats, gn_args(offsets, N, planes, groups, samples, dtype, V, leakiness), weight, bias,
+                                      eps, act, temp, as_stream(stream));
+  });
+}
+
+int scn_group_norm_backward(const void *x, const void *d_y, void *d_x, const float *stats, const int64_t *offsets,
+                            const float *weight, const float *bias, float *d_weight, float *d_bias, int act, double leakiness,
+                            int64_t N, int planes, int groups, int64_t samples, int dtype, void *temp, size_t temp_bytes,
+                            void *stream) {
+  if (int e = gn_check(N, planes, groups, samples, dtype, act)) return e;
+  SCN_REQUIRE(stats && offsets && (N == 0 || (x && d_y && d_x)), "group norm: pointers");
+  SCN_REQUIRE(temp && temp_bytes >= scn_group_norm_temp_bytes(N, planes, groups, samples, dtype, 1), "group norm: workspace");
+  return gn_dispatch(dtype, planes, [&](auto t, auto v) {
+    constexpr int V = decltype(v)::value;
+    return gn_backward<decltype(t), V>(x, d_y, d_x, stats, gn_args(offsets, N, planes, groups, samples, dtype, V, leakiness), weight,
+                                       bias, d_weight, d_bias, act, temp, as_stream(stream));
+  });
+}
+
+}  // extern "C"

@@ -15,14 +15,16 @@ from .containers import (AddTable, ConcatTable, Identity, JoinConcatTable, JoinT
                          ResidualConcatTable, Sequential)
 from .conv import Convolution, Deconvolution, SubmanifoldConvolution, ValidConvolution  # noqa: E402,F401
 from .io import InputLayer, OutputLayer  # noqa: E402,F401
-from .norm import BatchNormalization, BatchNormLeakyReLU, BatchNormReLU  # noqa: E402,F401
+from .norm import (BatchNormalization, BatchNormLeakyReLU, BatchNormReLU, GroupNormalization, GroupNormLeakyReLU,  # noqa: E402,F401
+                   GroupNormReLU, GroupNormSiLU)
+from .pointwise import Dropout, FusedNetworkInNetwork  # noqa: E402,F401
 from .tensor import Metadata, SparseConvNetTensor, optionalTensor, optionalTensorReturn, toLongTensor  # noqa: E402,F401
 from .unet import UNet  # noqa: E402,F401
 from .utils import add_feature_planes, upsample_feature  # noqa: E402,F401
 
 _OUT_OF_SCOPE = (
     "Tanh Sigmoid ReLU LeakyReLU ELU SELU BatchNormELU AveragePooling MeanOnlyBNLeakyReLU "
-    "ClassificationTrainValidate DenseToSparse Dropout BatchwiseDropout FullConvolution TransposeConvolution "
+    "ClassificationTrainValidate DenseToSparse BatchwiseDropout FullConvolution TransposeConvolution "
     "InputBatch BLInputLayer BLOutputLayer InputLayerInput MaxPooling PermutohedralSubmanifoldConvolution "
     "RandomizedStrideConvolution RandomizedStrideMaxPooling SparseToDense Sparsify spectral_norm UnPooling "
     "ShapeContext MultiscaleShapeContext SparseVggNet SparseResNet FullyConvolutionalNet").split()

@@ -4,9 +4,13 @@ Operator API of sparseconvnet/batchNormalization.py:13-161: eps 1e-4, momentum 0
 reference's convention running = momentum*running + (1-momentum)*batch,
 `leakiness` 0 = ReLU, 1 = no activation; buffers `running_mean`/`running_var`,
 parameters `weight`/`bias`.
+
+GroupNormalization beside it (not in the reference): statistics of groups of planes over the sites of each SAMPLE, the
+same in training and evaluation, with the activation inside.
 """
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 from torch.nn import Module, Parameter
 
 from .. import SCN
@@ -126,3 +130,97 @@ class BatchNormLeakyReLU(BatchNormalization):
 
     def _name(self):
         return "BatchNormLeakyReLU"
+
+
+class _GroupNormFunction(Function):
+    @staticmethod
+    def forward(ctx, features, weight, bias, offsets, eps, groups, activation, leakiness):
+        out = like_empty(features)
+        stats = torch.empty(0, dtype=torch.float32, device=features.device)
+        SCN.GroupNormalization_updateOutput(features, out, stats, offsets, weight, bias, eps, groups, activation, leakiness)
+        ctx.args = groups, activation, leakiness
+        ctx.save_for_backward(features, weight, bias, offsets, stats)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        features, weight, bias, offsets, stats = ctx.saved_tensors
+        grad_input = like_empty(grad_output)
+        grad_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
+        grad_bias = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
+        SCN.GroupNormalization_backward(features, grad_input, grad_output, stats, offsets, weight, bias, grad_weight, grad_bias,
+                                        *ctx.args)
+        return (grad_input, grad_weight, grad_bias) + (None,) * 5
+
+
+class GroupNormalization(Module):
+    """(not in the reference) ``nGroups`` groups of consecutive planes, each normalised over its planes and the sites of one sample,
+    then scaled, shifted and activated in the same pass: ``activation`` "leaky_relu" with ``leakiness`` (0 = ReLU, 1 = none, as
+    BatchNormalization), "silu" or "gelu".  Independent of the other samples of a batch and of whether the module is training.
+    float32, bfloat16 or float16 features; ``weight`` / ``bias`` are float32 or of the features' type."""
+
+    def __init__(self, nPlanes, nGroups, eps=1e-4, affine=True, leakiness=1, activation="leaky_relu"):
+        Module.__init__(self)
+        if nGroups < 1 or nPlanes < 1 or nPlanes % nGroups:
+            raise ValueError("GroupNormalization: %d planes do not divide into %d groups" % (nPlanes, nGroups))
+        SCN._activation("GroupNormalization", activation)
+        self.nPlanes, self.nGroups, self.eps = nPlanes, nGroups, eps
+        self.affine, self.leakiness, self.activation = affine, leakiness, activation
+        if affine:
+            self.weight = Parameter(torch.ones(nPlanes))
+            self.bias = Parameter(torch.zeros(nPlanes))
+
+    def forward(self, input):
+        features = input.features
+        if features.dim() != 2 or features.size(1) != self.nPlanes:
+            raise RuntimeError("GroupNormalization(%d): features %s" % (self.nPlanes, tuple(features.shape)))
+        weight, bias = optionalTensor(self, "weight"), optionalTensor(self, "bias")
+        if weight.dtype != torch.float32 and weight.dtype == features.dtype:
+            weight, bias = weight.float(), bias.float()
+        offsets = input.metadata.sampleOffsets(input.spatial_size)
+        if features.size(0) != input.metadata.getNActive(input.spatial_size):
+            raise RuntimeError("GroupNormalization: %d rows of features for %d sites"
+                               % (features.size(0), input.metadata.getNActive(input.spatial_size)))
+        output = SparseConvNetTensor(metadata=input.metadata, spatial_size=input.spatial_size)
+        output.features = apply_function(_GroupNormFunction, features, weight, bias, offsets, self.eps, self.nGroups, self.activation,
+                                         self.leakiness)
+        return output
+
+    def input_spatial_size(self, out_size):
+        return out_size
+
+    def _name(self):
+        return "GroupNorm"
+
+    def __repr__(self):
+        s = "%s(%d,%d,eps=%s,affine=%s" % (self._name(), self.nPlanes, self.nGroups, self.eps, self.affine)
+        if self.activation != "leaky_relu":
+            s += ",activation=%s" % self.activation
+        elif self.leakiness > 0 and type(self) is not GroupNormReLU:
+            s += ",leakiness=%s" % self.leakiness
+        return s + ")"
+
+
+class GroupNormReLU(GroupNormalization):
+    def __init__(self, nPlanes, nGroups, eps=1e-4):
+        GroupNormalization.__init__(self, nPlanes, nGroups, eps, True, 0)
+
+    def _name(self):
+        return "GroupNormReLU"
+
+
+class GroupNormLeakyReLU(GroupNormalization):
+    def __init__(self, nPlanes, nGroups, eps=1e-4, leakiness=0.333):
+        GroupNormalization.__init__(self, nPlanes, nGroups, eps, True, leakiness)
+
+    def _name(self):
+        return "GroupNormLeakyReLU"
+
+
+class GroupNormSiLU(GroupNormalization):
+    def __init__(self, nPlanes, nGroups, eps=1e-4):
+        GroupNormalization.__init__(self, nPlanes, nGroups, eps, True, activation="silu")
+
+    def _name(self):
+        return "GroupNormSiLU"
