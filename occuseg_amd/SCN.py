@@ -2029,6 +2029,10 @@ def rng_take(state):
     return used
 
 
+def factor_dtype(features):
+    return torch.float32 if features.dtype == torch.float32 else torch.int16
+
+
 def _linear_args(what, features, weight, bias):
     code = _pointwise(what, features, weight, bias)
     if weight.dim() != 2 or weight.size(0) < 1 or weight.size(1) < 1 or features.size(1) != weight.size(0):
@@ -2041,7 +2045,8 @@ def _linear_args(what, features, weight, bias):
 def FusedNetworkInNetwork_updateOutput(input_features, output_features, weight, bias, residual, activation, leakiness, p, rng,
                                        factor=None):
     """output = residual + dropout(act(input @ weight + bias)) in one kernel.  ``residual`` None: none; ``p`` 0: no dropout, ``rng``
-    None.  ``factor`` (an empty tensor, training) receives d output / d (input @ weight + bias) for the backward pass."""
+    None.  ``factor`` (an empty tensor of factor_dtype(input), training) receives d output / d (input @ weight + bias) for the backward
+    pass: float32, or 16-bit codes beside 16-bit features."""
     what = "FusedNetworkInNetwork_updateOutput"
     code, N, Ci, Co = _linear_args(what, input_features, weight, bias)
     act, p = _activation(what, activation), _drop_p(what, p)
@@ -2057,6 +2062,8 @@ def FusedNetworkInNetwork_updateOutput(input_features, output_features, weight, 
     with _on(x):
         output_features.resize_(N, Co)
         if factor is not None:
+            if factor.dtype != factor_dtype(x) or factor.device != x.device:
+                raise RuntimeError("occuseg_amd.SCN.%s: factor must be %s" % (what, factor_dtype(x)))
             factor.resize_(N, Co)
         ev = _prof_begin()
         check(_lib_().scn_linear_forward(ptr(x), ld, ptr(weight.contiguous()), ptr(bias), ptr(res), ld_res, ptr(output_features),
@@ -2066,13 +2073,17 @@ def FusedNetworkInNetwork_updateOutput(input_features, output_features, weight, 
     return float(N) * Ci * Co
 
 
-def FusedNetworkInNetwork_backward(input_features, d_input_features, d_output_features, weight, d_weight, d_bias, factor=None):
-    """d_input (None: not wanted), d_weight and d_bias (None: not wanted) are assigned; ``factor`` as the forward pass left it, None:
-    the pass had neither activation nor dropout.  The residual's gradient is d_output itself."""
+def FusedNetworkInNetwork_backward(input_features, d_input_features, d_output_features, weight, d_weight, d_bias, activation, leakiness,
+                                   p, factor=None):
+    """d_input (None: not wanted), d_weight and d_bias (None: not wanted) are assigned; activation, leakiness and p are the forward
+    pass's, ``factor`` as it left it; None: it had neither activation nor dropout.  The residual's gradient is d_output itself."""
     what = "FusedNetworkInNetwork_backward"
     code, N, Ci, Co = _linear_args(what, input_features, weight, None)
-    _pointwise(what, d_output_features, input_features, factor)
-    if tuple(d_output_features.shape) != (N, Co) or (factor is not None and tuple(factor.shape) != (N, Co)):
+    act, p, leakiness = _activation(what, activation), _drop_p(what, p), float(leakiness)
+    _pointwise(what, d_output_features, input_features)
+    if tuple(d_output_features.shape) != (N, Co) or (factor is not None and not (
+            tuple(factor.shape) == (N, Co) and factor.dtype == factor_dtype(input_features) and factor.is_contiguous()
+            and factor.device == input_features.device)):
         raise RuntimeError("occuseg_amd.SCN.%s: shapes" % what)
     x, ldx = _rows(input_features)
     dy, ld_dy = _rows(d_output_features)
@@ -2082,8 +2093,8 @@ def FusedNetworkInNetwork_backward(input_features, d_input_features, d_output_fe
         if d_input_features is not None:
             d_input_features.resize_(N, Ci)
             ev = _prof_begin()
-            check(lib.scn_linear_dinput(ptr(dy), ld_dy, ptr(factor), ptr(weight.contiguous()), ptr(d_input_features), N, Ci, Co, code,
-                                        stream()))
+            check(lib.scn_linear_dinput(ptr(dy), ld_dy, ptr(factor), ptr(weight.contiguous()), ptr(d_input_features), N, Ci, Co, act,
+                                        leakiness, p, code, stream()))
             _prof_end(ev, "linear_dx", 2.0 * N * Ci * Co, es * (N * (Ci + Co * (1 + (factor is not None))) + Ci * Co), (N, Ci, Co))
         if d_weight is not None:
             d_weight.resize_(Ci, Co)
@@ -2092,8 +2103,8 @@ def FusedNetworkInNetwork_backward(input_features, d_input_features, d_output_fe
             tb = lib.scn_linear_dweight_temp_bytes(N, Ci, Co)
             temp = torch.empty(tb, dtype=torch.uint8, device=x.device)
             ev = _prof_begin()
-            check(lib.scn_linear_dweight(ptr(x), ldx, ptr(dy), ld_dy, ptr(factor), ptr(d_weight), ptr(d_bias), N, Ci, Co, code,
-                                         ptr(temp), tb, stream()))
+            check(lib.scn_linear_dweight(ptr(x), ldx, ptr(dy), ld_dy, ptr(factor), ptr(d_weight), ptr(d_bias), N, Ci, Co, act,
+                                         leakiness, p, code, ptr(temp), tb, stream()))
             _prof_end(ev, "linear_dw", 2.0 * N * Ci * Co, es * (N * (Ci + Co * (1 + (factor is not None))) + Ci * Co), (N, Ci, Co))
 
 

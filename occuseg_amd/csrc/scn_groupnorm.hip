@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(256)
   const int span = (int)(r1 - r0) * a.C;
   const T *p = x + r0 * a.C;
   T *o = y + r0 * a.C;
-  constexpr bool EXACT = sizeof(T) == 4;
+  constexpr bool FINE = sizeof(T) == 4;
   for (int q = threadIdx.x; q < a.step; q += 256) {
     float mean[V], w[V], b[V];
 #pragma unroll
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(256)
     gn_walk<4, T, V>(p, span, q, a.step, [&](int i, int n, const Pack<T, V> &v) {
       Pack<T, V> r;
 #pragma unroll
-      for (int j = 0; j < V; ++j) r.v[j] = (T)act_value<ACT, EXACT>(fmaf((float)v.v[j] - mean[j], w[j], b[j]), a.leak);
+      for (int j = 0; j < V; ++j) r.v[j] = (T)act_value<ACT, FINE>(fmaf((float)v.v[j] - mean[j], w[j], b[j]), a.leak);
       gn_store<T, V>(o + i, n, r);
     });
   }
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(256)
   if (!gn_chunk(a, blockIdx.x, s, r0, r1)) return;
   const int span = (int)(r1 - r0) * a.C, E = a.step * V;
   const T *p = x + r0 * a.C, *g = dy + r0 * a.C;
-  constexpr bool EXACT = sizeof(T) == 4;
+  constexpr bool FINE = sizeof(T) == 4;
   for (int q = threadIdx.x; q < a.step; q += 256) {
     float mean[V], rstd[V], w[V], b[V], s1[V], s2[V];
 #pragma unroll
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float c = (float)v.v[j] - mean[j];
-        const float dz = j < n ? (float)d.v[j] * act_slope<ACT, EXACT>(fmaf(c, w[j], b[j]), a.leak) : 0.f;
+        const float dz = j < n ? (float)d.v[j] * act_slope<ACT, FINE>(fmaf(c, w[j], b[j]), a.leak) : 0.f;
         s1[j] += dz;
         s2[j] = fmaf(dz, c * rstd[j], s2[j]);
       }
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(256)
   const int span = (int)(r1 - r0) * a.C;
   const T *p = x + r0 * a.C, *g = dy + r0 * a.C;
   T *o = dx + r0 * a.C;
-  constexpr bool EXACT = sizeof(T) == 4;
+  constexpr bool FINE = sizeof(T) == 4;
   for (int q = threadIdx.x; q < a.step; q += 256) {
     float mean[V], rstd[V], w[V], b[V], m1[V], m2[V];
 #pragma unroll
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float c = (float)v.v[j] - mean[j];
-        const float dz = (float)d.v[j] * act_slope<ACT, EXACT>(fmaf(c, w[j], b[j]), a.leak);
+        const float dz = (float)d.v[j] * act_slope<ACT, FINE>(fmaf(c, w[j], b[j]), a.leak);
         r.v[j] = (T)(fmaf(dz, w[j], -m1[j]) - c * m2[j]);
       }
       gn_store<T, V>(o + i, n, r);

@@ -17,32 +17,31 @@
 namespace scn {
 
 // ------------------------------------------------------------------- dropout ---
-// One launch, every element read and written once; the mask is made of the counter (20 32x32 products per 4 elements, behind the
-// loads of a kernel that is HBM bound).  A thread's item: Q quads of planes of one site; `items` a row.  It keeps (row, item) by
-// steps of (drow, ditem): no division.
+// Every element read and written once; the mask is made of the counter.  A thread keeps its planes -- Q quads -- and walks the
+// sites, `rows` of a step at a time: the products of the counter that belong to the planes are made once.
 template <class T, int Q, bool WHOLE>
 __global__ void __launch_bounds__(256)
-    k_dropout(const T *x, int64_t ldx, T *y, int64_t N, int C, int items, int64_t drow, int ditem, uint32_t threshold, float scale,
-              const int64_t *rng) {
-  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  int64_t row = first / items;
-  int item = (int)(first - row * items);
+    k_dropout(const T *x, int64_t ldx, T *y, int64_t N, int C, int items, int rows, uint32_t threshold, float scale, const int64_t *rng) {
+  const int item = rows > 1 ? (int)threadIdx.x % items : (int)(blockIdx.y * 256 + threadIdx.x);
+  const int sub = rows > 1 ? (int)threadIdx.x / items : 0;
+  if (item >= items || sub >= rows) return;
   const RngKey key = rng_key(rng);
-  for (; row < N; row += drow, item += ditem) {
-    if (item >= items) {
-      item -= items;
-      if (++row >= N) break;
-    }
-    const int c = item * 4 * Q, n = WHOLE ? 4 * Q : min(4 * Q, C - c);
+  const int c = item * 4 * Q, n = WHOLE ? 4 * Q : min(4 * Q, C - c);
+  PhiloxPlane plane[Q];
+#pragma unroll
+  for (int u = 0; u < Q; ++u) plane[u] = philox_plane(key, (uint32_t)(item * Q + u));
+  const int64_t step = (int64_t)gridDim.x * rows;
+  for (int64_t row = (int64_t)blockIdx.x * rows + sub; row < N; row += step) {
     const T *p = x + row * ldx + c;
     Pack<T, 4 * Q> v;
     if (n == 4 * Q) v = load_pack<T, 4 * Q>(p);
     else
 #pragma unroll
       for (int j = 0; j < 4 * Q; ++j) v.v[j] = j < n ? p[j] : (T)0.f;
+    const PhiloxSite site = philox_site(key, (uint32_t)row);
 #pragma unroll
     for (int u = 0; u < Q; ++u) {
-      const Words w = philox(key, (uint32_t)(item * Q + u), (uint32_t)row);
+      const Words w = philox(key, plane[u], site);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v.v[4 * u + j] = w.w[j] >= threshold ? (T)((float)v.v[4 * u + j] * scale) : (T)0.f;
     }
@@ -81,13 +80,25 @@ __device__ __forceinline__ floatx4 mma(const halfx8 &a, const halfx8 &b, const f
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// n of the V elements at p, zeros behind them
+// n of the V elements at p, zeros behind them (16-bit ones packed as they come, or each would keep a register of its own)
 template <class T, int V>
 __device__ __forceinline__ Pack<T, V> load_some(const T *p, int n) {
   if (n >= V) return load_pack<T, V>(p);
   Pack<T, V> r;
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t *q = (const uint16_t *)p;
+    uint32_t w[V / 2];
 #pragma unroll
-  for (int j = 0; j < V; ++j) r.v[j] = j < n ? p[j] : (T)0.f;
+    for (int j = 0; j < V / 2; ++j) {
+      w[j] = 2 * j < n ? q[2 * j] : 0u;
+      if (2 * j + 1 < n) w[j] |= (uint32_t)q[2 * j + 1] << 16;
+      asm("" : "+v"(w[j]));
+    }
+    __builtin_memcpy(&r, w, sizeof(r));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) r.v[j] = j < n ? p[j] : (T)0.f;
+  }
   return r;
 }
 template <class T, int V>
@@ -99,8 +110,26 @@ __device__ __forceinline__ void store_some(T *p, const Pack<T, V> &v, int n) {
       if (j < n) p[j] = v.v[j];
 }
 
+// What the backward pass needs of activation and mask, one value per output: f = dy / d(x W + b).  fp32: f itself.  16-bit features:
+// rounding f to them, then dy f to them, would make the second of these roundings twice; 16 bits of fixed point are finer.
+//   FACTOR_FIXED  f = up q 2^-14, up = 1 / (1 - p); |slope| <= 1.13 for the smooth activations; q = -2^15: NaN
+//   FACTOR_SIGN   q = 2: f = up, 1: up leak, 0: dropped     (leaky ReLU, whose slope may be any number)
+enum { FACTOR_NONE, FACTOR_FLOAT, FACTOR_FIXED, FACTOR_SIGN };
+template <class T> struct FactorOf { using type = int16_t; };
+template <> struct FactorOf<float> { using type = float; };
+
+struct FactorScale {
+  float unit, up, low;
+};
+template <int FACTOR, class Q>
+__device__ __forceinline__ float factor_value(Q q, const FactorScale &s) {
+  if constexpr (FACTOR == FACTOR_FLOAT) return (float)q;
+  if constexpr (FACTOR == FACTOR_SIGN) return q == 2 ? s.up : q == 1 ? s.low : 0.f;
+  return (int)q == -32768 ? __builtin_nanf("") : (float)(int)q * s.unit;
+}
+
 struct LinearArgs {
-  const void *in, *scale;  // rows [N, K] at ld_in elements; MODE 1: times scale [N, K] (may be NULL)
+  const void *in, *factor_in;  // rows [N, K] at ld_in elements; MODE 1: times the factors [N, K]
   int64_t ld_in;
   const void *weight;  // MODE 0: [K, M], MODE 1: [M, K]
   const void *bias, *residual;
@@ -112,8 +141,20 @@ struct LinearArgs {
   int groups, chunk_groups;  // k-groups in all, and per pass through LDS
   int col_blocks, row_blocks;
   uint32_t threshold;
-  float leak, keep_scale;
+  float leak, up;
+  FactorScale scale;
 };
+
+// one output's activation, mask, residual; a kept or dropped element's factor
+template <class T, int ACT>
+__device__ __forceinline__ float epilogue(float z, bool keep, float res, const LinearArgs &a, typename FactorOf<T>::type &factor) {
+  float value, slope;
+  act_value_slope<ACT, sizeof(T) == 4>(z, a.leak, value, slope);
+  if constexpr (sizeof(T) == 4) factor = keep ? slope * a.up : 0.f;
+  else if (ACT == SCN_ACT_LEAKY) factor = keep ? (z > 0 ? 2 : 1) : 0;
+  else factor = !keep ? 0 : slope == slope ? (int16_t)(int)rintf(slope * 16384.f) : -32768;
+  return (keep ? value * a.up : 0.f) + res;
+}
 
 constexpr int LIN_ROWS = 128;  // rows of a workgroup's tile: 4 waves x 2 x 16
 
@@ -123,16 +164,16 @@ __device__ __forceinline__ int tile_col(int t, int i) {
   return sizeof(T) == 4 ? 16 * t + i : 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3);
 }
 
-// MODE 0: forward with the epilogue.  MODE 1: dx.
+// MODE 0: forward with the epilogue, X its activation.  MODE 1: dx, X how the factors are stored.
 // A workgroup holds the weights of NT x 16 output planes in LDS -- all of K, once, if they fit (then its waves walk their rows
 // without a barrier), else `chunk_groups` at a time -- and walks the row tiles row_block, row_block + row_blocks, ...
-template <class T, int NT, int MODE, int ACT>
-__global__ void __launch_bounds__(256) k_linear(LinearArgs a) {
-  constexpr int V = Elem<T>::V, KG = 4 * V;
-  constexpr bool EXACT = sizeof(T) == 4;
+template <class T, int NT, int MODE, int X>
+__global__ void __launch_bounds__(256, 3) k_linear(LinearArgs a) {
+  constexpr int V = Elem<T>::V, KG = 4 * V, STAGE_UNROLL = MODE == 0 ? 4 : 1;
   using F = typename Frag<T>::type;
+  using Q = typename FactorOf<T>::type;
   extern __shared__ char smem[];
-  F *wl = (F *)smem;  // [tile][k-group of the chunk][lane]
+  F *wl = (F *)smem;  // [k-group of the chunk][tile][lane]
   float *bl = (float *)(wl + (size_t)NT * a.chunk_groups * 64);
   const int lane = lane_id(), wave = threadIdx.x >> 6, li = lane & 15, lq = lane >> 4;
   // the column blocks of one row block run on one XCD (workgroup ids go round the 8 of them): its rows come from that L2 once
@@ -147,13 +188,15 @@ __global__ void __launch_bounds__(256) k_linear(LinearArgs a) {
     rb = id / a.col_blocks;
   }
   const int m0 = cb * NT * 16;
-  const T *in = (const T *)a.in, *sc = (const T *)a.scale, *wt = (const T *)a.weight;
+  const T *in = (const T *)a.in, *wt = (const T *)a.weight;
+  const Q *fi = (const Q *)a.factor_in;
   if (MODE == 0 && threadIdx.x < NT * 16) {
     const int m = m0 + threadIdx.x;
     bl[threadIdx.x] = a.bias && m < a.M ? (float)((const T *)a.bias)[m] : 0.f;
   }
   RngKey key = {};
   if (MODE == 0 && a.threshold) key = rng_key(a.rng);
+  const int full = a.K / KG;  // k-groups that lie inside the rows
   bool staged = false;
   const int64_t tiles = (a.N + LIN_ROWS - 1) / LIN_ROWS;
   for (int64_t tile = rb; tile < tiles; tile += a.row_blocks) {
@@ -164,122 +207,203 @@ __global__ void __launch_bounds__(256) k_linear(LinearArgs a) {
       for (int t = 0; t < NT; ++t) acc[u][t] = floatx4{0.f, 0.f, 0.f, 0.f};
     const int64_t row0 = tile * LIN_ROWS + wave * 32 + li;
     // (rows behind the last are read as the last and not written)
-    const T *p[2] = {in + min(row0, a.N - 1) * a.ld_in + lq * V, in + min(row0 + 16, a.N - 1) * a.ld_in + lq * V};
-    const T *ps[2] = {nullptr, nullptr};
-    if (MODE == 1 && sc) {
-      ps[0] = sc + min(row0, a.N - 1) * a.K + lq * V;
-      ps[1] = sc + min(row0 + 16, a.N - 1) * a.K + lq * V;
+    const int64_t rr[2] = {min(row0, a.N - 1), min(row0 + 16, a.N - 1)};
+    const T *p[2] = {in + rr[0] * a.ld_in + lq * V, in + rr[1] * a.ld_in + lq * V};
+    const Q *pf[2] = {nullptr, nullptr};
+    if (MODE == 1 && X != FACTOR_NONE) {
+      pf[0] = fi + rr[0] * a.K + lq * V;
+      pf[1] = fi + rr[1] * a.K + lq * V;
     }
     for (int g0 = 0; g0 < a.groups; g0 += a.chunk_groups) {
       const int ng = min(a.chunk_groups, a.groups - g0);
       if (!staged || a.groups > a.chunk_groups) {
         __syncthreads();
+#pragma unroll STAGE_UNROLL
         for (int e = threadIdx.x; e < NT * ng * 64; e += 256) {
-          const int l = e & 63, g = (e >> 6) % ng, t = (e >> 6) / ng;
+          const int l = e & 63, t = (e >> 6) % NT, g = (e >> 6) / NT;
           const int m = m0 + tile_col<T>(t, l & 15), k = (g0 + g) * KG + (l >> 4) * V;
           Pack<T, V> v;
-          if (MODE == 1) {
-            if (m < a.M) v = load_some<T, V>(wt + (int64_t)m * a.K + k, a.K - k);
-            else
-#pragma unroll
-              for (int j = 0; j < V; ++j) v.v[j] = (T)0.f;
-          } else {
+          if (MODE == 1) v = load_some<T, V>(wt + (int64_t)m * a.K + k, m < a.M ? a.K - k : 0);
+          else
 #pragma unroll
             for (int j = 0; j < V; ++j) v.v[j] = m < a.M && k + j < a.K ? wt[(int64_t)(k + j) * a.M + m] : (T)0.f;
-          }
-          __builtin_memcpy(&wl[((size_t)t * a.chunk_groups + g) * 64 + l], &v, 16);
+          __builtin_memcpy(&wl[e], &v, 16);
         }
         __syncthreads();
         staged = true;
       }
-      auto load_row = [&](int u, int g) __attribute__((always_inline)) {
-        const int k = (g0 + g) * KG, left = a.K - k - lq * V;
-        Pack<T, V> v = left >= V ? load_pack<T, V>(p[u] + k) : load_some<T, V>(p[u] + k, left);
-        if (MODE == 1 && sc) {
-          const Pack<T, V> f = left >= V ? load_pack<T, V>(ps[u] + k) : load_some<T, V>(ps[u] + k, left);
+      // G k-groups: their rows are requested together, then multiplied
+      auto batch = [&](auto count, auto whole, int g) __attribute__((always_inline)) {
+        constexpr int G = decltype(count)::value;
+        constexpr bool WHOLE = decltype(whole)::value;
+        Pack<T, V> v[G][2];
+        Pack<Q, V> f[G][2];
 #pragma unroll
-          for (int j = 0; j < V; ++j) v.v[j] = (T)((float)v.v[j] * (float)f.v[j]);
+        for (int i = 0; i < G; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int k = (g0 + g + i) * KG, left = a.K - k - lq * V;
+            v[i][u] = WHOLE ? load_pack<T, V>(p[u] + k) : load_some<T, V>(p[u] + k, left);
+            if constexpr (MODE == 1 && X != FACTOR_NONE) f[i][u] = WHOLE ? load_pack<Q, V>(pf[u] + k) : load_some<Q, V>(pf[u] + k, left);
+          }
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          F b[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if constexpr (MODE == 1 && X != FACTOR_NONE)
+#pragma unroll
+              for (int j = 0; j < V; ++j) v[i][u].v[j] = (T)((float)v[i][u].v[j] * factor_value<X>(f[i][u].v[j], a.scale));
+            __builtin_memcpy(&b[u], &v[i][u], 16);
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const F w = wl[((g + i) * NT + t) * 64 + lane];
+            acc[0][t] = mma(w, b[0], acc[0][t]);
+            acc[1][t] = mma(w, b[1], acc[1][t]);
+          }
+          if (NT == 8) __builtin_amdgcn_sched_barrier(0);  // (one k-group's weights in registers at a time)
         }
-        F r;
-        __builtin_memcpy(&r, &v, 16);
-        return r;
       };
-#pragma unroll 4
-      for (int g = 0; g < ng; ++g) {
-        const F b0 = load_row(0, g), b1 = load_row(1, g);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const F w = wl[((size_t)t * a.chunk_groups + g) * 64 + lane];
-          acc[0][t] = mma(w, b0, acc[0][t]);
-          acc[1][t] = mma(w, b1, acc[1][t]);
-        }
-      }
+      const int nf = min(ng, full - g0);
+      int g = 0;
+      if (NT < 8)
+        for (; g + 4 <= nf; g += 4) batch(std::integral_constant<int, 4>(), std::true_type(), g);
+      for (; g + 2 <= nf; g += 2) batch(std::integral_constant<int, 2>(), std::true_type(), g);
+      if (g < nf) batch(std::integral_constant<int, 1>(), std::true_type(), g++);
+      if (g < ng) batch(std::integral_constant<int, 1>(), std::false_type(), g);
     }
     constexpr int TP = V / 4;  // tiles per 16-byte store
+    PhiloxSite site[2] = {};
+    if (MODE == 0 && a.threshold) {
+      site[0] = philox_site(key, (uint32_t)row0);
+      site[1] = philox_site(key, (uint32_t)row0 + 16);
+    }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int64_t row = row0 + 16 * u;
-      if (row >= a.N) continue;
+    for (int t = 0; t < NT; t += TP) {
+      const int cl = tile_col<T>(t, 4 * lq), m = m0 + cl;
+      if (m >= a.M) continue;
+      PhiloxPlane plane[TP] = {};
+      if (MODE == 0 && a.threshold)
 #pragma unroll
-      for (int t = 0; t < NT; t += TP) {
-        const int cl = tile_col<T>(t, 4 * lq), m = m0 + cl;
-        if (m >= a.M) continue;
+        for (int q = 0; q < TP; ++q) plane[q] = philox_plane(key, (uint32_t)((m >> 2) + q));
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int64_t row = row0 + 16 * u;
+        if (row >= a.N) continue;
         Pack<T, V> y;
-        if (MODE == 1) {
+        if constexpr (MODE == 1) {
 #pragma unroll
           for (int j = 0; j < V; ++j) y.v[j] = (T)acc[u][t + j / 4][j & 3];
         } else {
-          Pack<T, V> f, res;
+          Pack<T, V> res;
+          Pack<Q, V> f;
           if (a.residual) res = load_some<T, V>((const T *)a.residual + row * a.ld_res + m, a.M - m);
 #pragma unroll
           for (int q = 0; q < TP; ++q) {
             Words w;
-            if (a.threshold) w = philox(key, (uint32_t)((m >> 2) + q), (uint32_t)row);
+            if (a.threshold) w = philox(key, plane[q], site[u]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float value, slope;
-              act_value_slope<ACT, EXACT>(acc[u][t + q][j] + bl[cl + 4 * q + j], a.leak, value, slope);
-              if (a.threshold) {
-                const bool keep = w.w[j] >= a.threshold;
-                value = keep ? value * a.keep_scale : 0.f;
-                slope = keep ? slope * a.keep_scale : 0.f;
-              }
-              if (a.residual) value += (float)res.v[4 * q + j];
-              y.v[4 * q + j] = (T)value;
-              f.v[4 * q + j] = (T)slope;
-            }
+            for (int j = 0; j < 4; ++j)
+              y.v[4 * q + j] = (T)epilogue<T, X>(acc[u][t + q][j] + bl[cl + 4 * q + j], !a.threshold || w.w[j] >= a.threshold,
+                                                 a.residual ? (float)res.v[4 * q + j] : 0.f, a, f.v[4 * q + j]);
           }
-          if (a.factor) store_some<T, V>((T *)a.factor + row * a.M + m, f, a.M - m);
+          if (a.factor) store_some<Q, V>((Q *)a.factor + row * a.M + m, f, a.M - m);
         }
         store_some<T, V>((T *)a.out + row * a.M + m, y, a.M - m);
       }
+      __builtin_amdgcn_sched_barrier(0);  // (one tile's epilogue at a time: all of them interleaved do not fit the registers)
     }
   }
 }
 
+// Up to R rows (a serving loop's single sites): bound by one trip to memory for the weights, which the tiles above would make with a
+// few workgroups in many steps.  A workgroup has 16 output planes; its threads share out the reduction, 16 bytes of a weight row
+// each, and join in the wave, then through LDS.
+template <class T, int R, int ACT>
+__global__ void __launch_bounds__(1024) k_linear_few(LinearArgs a) {
+  constexpr int V = Elem<T>::V, LC = 16 / V, PHASES = 1024 / LC;
+  __shared__ float red[16][R][16];
+  const int m0 = blockIdx.x * 16, cl = threadIdx.x % LC * V, m = m0 + cl;
+  const T *x = (const T *)a.in, *wt = (const T *)a.weight;
+  float acc[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[r][j] = 0.f;
+  for (int k = threadIdx.x / LC; k < a.K; k += PHASES) {
+    const Pack<T, V> w = load_some<T, V>(wt + (int64_t)k * a.M + m, a.M - m);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float xv = (float)x[min((int64_t)r, a.N - 1) * a.ld_in + k];
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[r][j] = fmaf(xv, (float)w.v[j], acc[r][j]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+#pragma unroll
+      for (int o = LC; o < 64; o <<= 1) acc[r][j] += __shfl_xor(acc[r][j], o);
+    }
+  if (lane_id() < LC)
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int j = 0; j < V; ++j) red[threadIdx.x >> 6][r][cl + j] = acc[r][j];
+  __syncthreads();
+  const int row = threadIdx.x >> 4, c = threadIdx.x & 15, mo = m0 + c;
+  if (row >= R || row >= a.N || mo >= a.M) return;
+  float z = 0.f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) z += red[w][row][c];
+  z += a.bias ? (float)((const T *)a.bias)[mo] : 0.f;
+  bool keep = true;
+  if (a.threshold) {
+    const RngKey key = rng_key(a.rng);
+    const Words w = philox(key, philox_plane(key, (uint32_t)mo >> 2), philox_site(key, (uint32_t)row));
+    keep = ((mo & 2) ? (mo & 1) ? w.w[3] : w.w[2] : (mo & 1) ? w.w[1] : w.w[0]) >= a.threshold;
+  }
+  typename FactorOf<T>::type f;
+  const float y = epilogue<T, ACT>(z, keep, a.residual ? (float)((const T *)a.residual)[row * a.ld_res + mo] : 0.f, a, f);
+  ((T *)a.out)[(int64_t)row * a.M + mo] = (T)y;
+  if (a.factor) ((typename FactorOf<T>::type *)a.factor)[(int64_t)row * a.M + mo] = f;
+}
+
 // ------------------------------------------------------------------- dweight ---
-// dW = x^T dz: the reduction runs over the rows, both operands are walked along their planes.  A wave's tile is 64 x 64: a lane
+// dW = x^T dz: the reduction runs over the rows, both operands are walked along their planes.  A wave's tile is 64 TI x 64: a lane
 // loads 4 consecutive planes of a row, which are its elements of four A (B) tiles with the planes interleaved by four -- fp32
-// needs nothing else; of 16-bit types eight rows are loaded and transposed in registers.  No LDS in the loop.
+// needs nothing else; of 16-bit types eight rows are loaded and transposed in registers.  No LDS in the loop.  Planes behind the last
+// are read as what follows in memory: they reach only results that are not stored.  Steps whose reads would leave a tensor are
+// loaded element by element (the last rows of the last slice).
 // Workgroup (slice, tile): four waves take the slice's row steps in turn, join through LDS and write one slab; slabs are added by
 // k_linear_dw_join in slice order.
 struct DwArgs {
-  const void *x, *dy, *scale;
+  const void *x, *dy, *factor;
   int64_t ldx, ld_dy, N;
   int Ci, Co, tiles_i, tiles_o, slices;
   int64_t slice_rows;
   float *slab;      // [slices][Ci][Co], then [slices][Co]
   int want_bias;
+  FactorScale scale;
 };
 
-template <class T>
-__global__ void __launch_bounds__(256) k_linear_dw(DwArgs a) {
+// rows r for which the 64 planes from c0 of rows up to r lie in the memory of a [N, C] tensor with rows at ld
+__device__ __forceinline__ int64_t rows_inside(int64_t N, int64_t ld, int C, int c_end) {
+  const int64_t room = (N - 1) * ld + C - c_end;
+  return room < 0 ? 0 : min(N, room / ld + 1);
+}
+
+template <class T, int TI, int FACTOR>
+__global__ void __launch_bounds__(256, 2) k_linear_dw(DwArgs a) {
   constexpr bool F32 = sizeof(T) == 4;
-  constexpr int ROWS = F32 ? 4 : 32;  // rows of one step
-  constexpr int RE = F32 ? 1 : 8;     // ... of one lane
+  constexpr int RE = F32 ? 4 : 8;  // rows of a lane in one step
+  constexpr int ROWS = 4 * RE;
   using F = typename Frag<T>::type;
-  __shared__ float red[2][64 * 64 + 64];
-  const int lane = lane_id(), wave = threadIdx.x >> 6, li = lane & 15, lq = lane >> 4;
+  using Q = typename FactorOf<T>::type;
+  __shared__ float red[TI * 64 * 64 + 64];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lq = lane >> 4;
   const int tiles = a.tiles_i * a.tiles_o;
   // (all tiles of a slice run on one XCD while its rows are in that L2)
   int slice, tile;
@@ -290,126 +414,154 @@ __global__ void __launch_bounds__(256) k_linear_dw(DwArgs a) {
     slice = blockIdx.x / tiles;
     tile = blockIdx.x % tiles;
   }
-  const int ci0 = tile / a.tiles_o * 64, co0 = tile % a.tiles_o * 64;
+  const int ci0 = tile / a.tiles_o * 64 * TI, co0 = tile % a.tiles_o * 64;
   const bool bias = a.want_bias && ci0 == 0;
   const int64_t r0 = slice * a.slice_rows, r1 = min(r0 + a.slice_rows, a.N);
-  const int ci = ci0 + 4 * li, co = co0 + 4 * li, ni = a.Ci - ci, no = a.Co - co;
-  const T *px = (const T *)a.x + ci, *pd = (const T *)a.dy + co, *ps = a.scale ? (const T *)a.scale + co : nullptr;
-  floatx4 acc[4][4], sums[4];
+  const int ci = ci0 + 4 * li, co = co0 + 4 * li, no = a.Co - co;
+  // a step's rows from scalar addresses, a lane's part of them from 32-bit offsets
+  const T *px = (const T *)a.x + ci0, *pd = (const T *)a.dy + co0;
+  const Q *pf = (const Q *)a.factor + co0;
+  const int lr = F32 ? lq : lq * RE;  // a lane's first row (fp32: a load of four whole rows; 16-bit: a lane's eight rows)
+  const unsigned ox = (unsigned)(lr * (int)a.ldx + 4 * li), od = (unsigned)(lr * (int)a.ld_dy + 4 * li), of = (unsigned)(lr * a.Co + 4 * li);
+  int64_t inside = min(rows_inside(a.N, a.ldx, a.Ci, ci0 + 64 * TI), rows_inside(a.N, a.ld_dy, a.Co, co0 + 64));
+  if (FACTOR != FACTOR_NONE) inside = min(inside, rows_inside(a.N, a.Co, a.Co, co0 + 64));
+  inside = min(inside, r1);
+  floatx4 acc[4 * TI][4], sums = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    sums[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-  }
-  for (int64_t r = r0 + wave * ROWS; r < r1; r += 4 * ROWS) {
-    Pack<T, 4> vx[RE], vd[RE];
+    for (int i = 0; i < 4 * TI; ++i) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  auto step = [&](auto whole, int64_t r) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    Pack<T, 4> vx[TI][RE], vd[RE];
+    Pack<Q, 4> vf[RE];
 #pragma unroll
     for (int e = 0; e < RE; ++e) {
-      const int64_t row = r + lq * RE + e;
-      const bool in = row < r1;
-      vx[e] = load_some<T, 4>(px + row * a.ldx, in ? ni : 0);
-      vd[e] = load_some<T, 4>(pd + row * a.ld_dy, in ? no : 0);
-      if (ps) {
-        const Pack<T, 4> f = load_some<T, 4>(ps + row * a.Co, in ? no : 0);
+      const int64_t row = r + (F32 ? 4 * e : e);
+      const bool in = row + lr < r1;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) vd[e].v[j] = (T)((float)vd[e].v[j] * (float)f.v[j]);
+      for (int t = 0; t < TI; ++t) {
+        const T *p = px + row * a.ldx + 64 * t;
+        vx[t][e] = WHOLE ? load_pack<T, 4>(p + ox) : load_some<T, 4>(p + ox, in ? a.Ci - ci - 64 * t : 0);
       }
+      const T *p = pd + row * a.ld_dy;
+      vd[e] = WHOLE ? load_pack<T, 4>(p + od) : load_some<T, 4>(p + od, in ? no : 0);
+      if constexpr (FACTOR != FACTOR_NONE) {
+        const Q *q = pf + row * a.Co;
+        vf[e] = WHOLE ? load_pack<Q, 4>(q + of) : load_some<Q, 4>(q + of, in ? no : 0);
+      }
+      if (!WHOLE) __builtin_amdgcn_sched_barrier(0);  // (a row at a time: nothing to gain, and fewer registers)
     }
+    if constexpr (FACTOR != FACTOR_NONE)
+#pragma unroll
+      for (int e = 0; e < RE; ++e)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vd[e].v[j] = (T)((float)vd[e].v[j] * factor_value<FACTOR>(vf[e].v[j], a.scale));
     if constexpr (F32) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int e = 0; e < RE; ++e) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[0].v[i], vd[0].v[j], acc[i][j], 0, 0, 0);
-      if (bias)
+        for (int i = 0; i < 4 * TI; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sums[0][j] += vd[0].v[j];
+          for (int j = 0; j < 4; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[i / 4][e].v[i & 3], vd[e].v[j], acc[i][j], 0, 0, 0);
+        if (bias)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sums[j] += vd[e].v[j];
+      }
     } else {
-      F fx[4], fd[4];
+      F fd[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          fx[j][e] = vx[e].v[j];
-          fd[j][e] = vd[e].v[j];
+        for (int e = 0; e < 8; ++e) fd[j][e] = vd[e].v[j];
+      if (bias)  // column sums: a product with ones in row j, so that the four tiles' sums share one result
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          F one;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) one[e] = li == j ? (T)1.f : (T)0.f;
+          sums = mma(one, fd[j], sums);
         }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4 * TI; ++i) {
+        F fx;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mma(fx[i], fd[j], acc[i][j]);
-      if (bias) {  // column sums: a product with ones, every row of the result the same
-        F one;
+        for (int e = 0; e < 8; ++e) fx[e] = vx[i / 4][e].v[i & 3];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) one[e] = (T)1.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sums[j] = mma(one, fd[j], sums[j]);
+        for (int j = 0; j < 4; ++j) acc[i][j] = mma(fx, fd[j], acc[i][j]);
       }
     }
-  }
-  // column 4 li + j: fp32 has it in sums[0][j] of the four lane quarters, 16-bit types in sums[j][0] of each of them
-  float bsum[4];
+  };
+  int64_t r = r0 + wave * ROWS;
+  for (; r + ROWS <= inside; r += 4 * ROWS) step(std::true_type(), r);
+  for (; r < r1; r += 4 * ROWS) step(std::false_type(), r);
+  // sums[j] of column 4 li + j: fp32 has parts of it in the four lane quarters, 16-bit types all of it in the first
+  if (F32)
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    bsum[j] = F32 ? sums[0][j] : sums[j][0];
-    if (F32) {
-      bsum[j] += __shfl_xor(bsum[j], 16);
-      bsum[j] += __shfl_xor(bsum[j], 32);
+    for (int j = 0; j < 4; ++j) {
+      sums[j] += __shfl_xor(sums[j], 16);
+      sums[j] += __shfl_xor(sums[j], 32);
     }
-  }
-  // waves 2, 3 hand over to 0, 1; then 1 to 0
+  // waves 1, 2, 3 hand over to wave 0, one after the other
+#pragma unroll 1
+  for (int w = 1; w < 4; ++w) {
+    if (wave == w) {
 #pragma unroll
-  for (int half = 2; half >= 1; half >>= 1) {
-    if (wave >= half && wave < 2 * half) {
-      float *d = red[wave - half];
+      for (int i = 0; i < 4 * TI; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *(floatx4 *)(d + ((i * 4 + j) * 64 + lane) * 4) = acc[i][j];
+        for (int j = 0; j < 4; ++j) *(floatx4 *)(red + ((i * 4 + j) * 64 + lane) * 4) = acc[i][j];
       if (lq == 0)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) d[4096 + 4 * li + j] = bsum[j];
+        for (int j = 0; j < 4; ++j) red[TI * 4096 + 4 * li + j] = sums[j];
     }
     __syncthreads();
-    if (wave < half) {
-      const float *d = red[wave];
+    if (wave == 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4 * TI; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += *(const floatx4 *)(d + ((i * 4 + j) * 64 + lane) * 4);
+        for (int j = 0; j < 4; ++j) acc[i][j] += *(const floatx4 *)(red + ((i * 4 + j) * 64 + lane) * 4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) bsum[j] += d[4096 + 4 * li + j];
+      for (int j = 0; j < 4; ++j) sums[j] += red[TI * 4096 + 4 * li + j];
     }
     __syncthreads();
   }
   if (wave != 0) return;
   float *slab = a.slab + (int64_t)slice * a.Ci * a.Co;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 4 * TI; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = ci0 + 16 * lq + 4 * r + i;  // A row 4 lq + r of tile i
+    for (int q = 0; q < 4; ++q) {
+      const int row = ci0 + 64 * (i / 4) + 16 * lq + 4 * q + (i & 3);  // A row 4 lq + q of tile i
       if (row < a.Ci && no > 0) {
-        Pack<float, 4> v = {{acc[i][0][r], acc[i][1][r], acc[i][2][r], acc[i][3][r]}};
+        Pack<float, 4> v = {{acc[i][0][q], acc[i][1][q], acc[i][2][q], acc[i][3][q]}};
         store_some<float, 4>(slab + (int64_t)row * a.Co + co, v, no);
       }
     }
   if (bias && lq == 0 && no > 0) {
-    Pack<float, 4> v = {{bsum[0], bsum[1], bsum[2], bsum[3]}};
+    Pack<float, 4> v = {{sums[0], sums[1], sums[2], sums[3]}};
     store_some<float, 4>(a.slab + (int64_t)a.slices * a.Ci * a.Co + (int64_t)slice * a.Co + co, v, no);
   }
 }
 
-// the slabs added in slice order; element e of [Ci * Co] then [Co]
+// the slabs added: wave w of 16 takes slabs w, w + 16, ..., then the waves in order; element e of [Ci * Co] then [Co]
 template <class T>
-__global__ void __launch_bounds__(256) k_linear_dw_join(const float *slab, int slices, int64_t nw, int nb, T *d_weight, T *d_bias) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= nw + nb) return;
-  const bool w = e < nw;
+__global__ void __launch_bounds__(1024) k_linear_dw_join(const float *slab, int slices, int64_t nw, int nb, T *d_weight, T *d_bias) {
+  __shared__ float red[16][64];
+  const int lane = lane_id(), wave = threadIdx.x >> 6;
+  const int64_t e = (int64_t)blockIdx.x * 64 + lane;
+  const bool in = e < nw + nb, w = e < nw;
   const float *p = w ? slab + e : slab + slices * nw + (e - nw);
   const int64_t step = w ? nw : nb;
   float s = 0.f;
+  if (in)
 #pragma unroll 8
-  for (int i = 0; i < slices; ++i) s += p[i * step];
+    for (int i = wave; i < slices; i += 16) s += p[i * step];
+  red[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || !in) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += red[i][lane];
   if (w) d_weight[e] = (T)s;
   else d_bias[e - nw] = (T)s;
 }
@@ -429,12 +581,12 @@ static int by_type(int dtype, F &&f) {
   return f((_Float16)0);
 }
 
-template <class T, int NT, int MODE, int ACT>
+template <class T, int NT, int MODE, int X>
 static int linear_launch(LinearArgs a, hipStream_t st) {
   constexpr int KG = 4 * Elem<T>::V, group_bytes = NT * 64 * 16;
   a.groups = (a.K + KG - 1) / KG;
   a.chunk_groups = a.groups;
-  if (a.groups * group_bytes > 49152) a.chunk_groups = 32768 / group_bytes;
+  if (a.groups * group_bytes > 61440) a.chunk_groups = 32768 / group_bytes;
   a.col_blocks = (a.M + NT * 16 - 1) / (NT * 16);
   const int64_t tiles = (a.N + LIN_ROWS - 1) / LIN_ROWS;
   int64_t rows = 1024 / a.col_blocks;
@@ -442,24 +594,58 @@ static int linear_launch(LinearArgs a, hipStream_t st) {
   if (a.groups > a.chunk_groups || rows > tiles) rows = tiles;  // (weights that do not stay: one tile a workgroup)
   a.row_blocks = (int)rows;
   const size_t lds = (size_t)a.chunk_groups * group_bytes + NT * 16 * 4;
-  k_linear<T, NT, MODE, ACT><<<(unsigned)(rows * a.col_blocks), 256, lds, st>>>(a);
+  k_linear<T, NT, MODE, X><<<(unsigned)(rows * a.col_blocks), 256, lds, st>>>(a);
   SCN_CHECK_LAUNCH();
   return 0;
 }
-template <class T, int MODE, int ACT>
+// wide column blocks read the rows least often; narrower ones while the chip is not full, or if they pad fewer planes
+template <class T, int MODE, int X>
 static int linear_by_width(const LinearArgs &a, hipStream_t st) {
-  if (a.M <= 32) return linear_launch<T, 2, MODE, ACT>(a, st);
-  if (a.M <= 64) return linear_launch<T, 4, MODE, ACT>(a, st);
-  return linear_launch<T, 8, MODE, ACT>(a, st);
+  const int64_t tiles = (a.N + LIN_ROWS - 1) / LIN_ROWS;
+  auto blocks = [&](int nt) { return (a.M + 16 * nt - 1) / (16 * nt); };
+  if (a.M <= 32 || tiles * blocks(4) < 256) return linear_launch<T, 2, MODE, X>(a, st);
+  if (a.M <= 64 || tiles * blocks(8) < 256 || blocks(4) < 2 * blocks(8)) return linear_launch<T, 4, MODE, X>(a, st);
+  return linear_launch<T, 8, MODE, X>(a, st);
+}
+template <class T, int ACT>
+static int linear_forward(const LinearArgs &a, hipStream_t st) {
+  if (a.N > 4) return linear_by_width<T, 0, ACT>(a, st);
+  const unsigned blocks = (unsigned)((a.M + 15) / 16);
+  if (a.N == 1) k_linear_few<T, 1, ACT><<<blocks, 1024, 0, st>>>(a);
+  else k_linear_few<T, 4, ACT><<<blocks, 1024, 0, st>>>(a);
+  SCN_CHECK_LAUNCH();
+  return 0;
 }
 
-// rows a slice of dW holds: enough slices to fill the chip with its tiles, no slice below 256 rows
+static FactorScale factor_scale(double leak, double p) {
+  const double up = 1.0 / (1.0 - p);
+  return FactorScale{(float)(up / 16384.0), (float)up, (float)(up * leak)};
+}
+// f(how the factors are stored)
+template <class T, class F>
+static int by_factor(const void *factor, int act, F &&f) {
+  if (!factor) return f(std::integral_constant<int, FACTOR_NONE>());
+  if constexpr (sizeof(T) == 4) return f(std::integral_constant<int, FACTOR_FLOAT>());
+  else return act == SCN_ACT_LEAKY ? f(std::integral_constant<int, FACTOR_SIGN>()) : f(std::integral_constant<int, FACTOR_FIXED>());
+}
+
+// planes a tile of dW takes of x: 128 read d_y and the factors half as often; with 16-bit features and factors that is more than the
+// registers hold
+template <class T, int FACTOR>
+constexpr bool dw_wide() { return sizeof(T) == 4 || FACTOR == FACTOR_NONE; }
+// row slices of dW: with its 64 x 64 tiles four workgroups a CU (two of the wide ones), no slice below 256 rows
 static int dw_slices(int64_t N, int n_in, int n_out) {
   const int64_t tiles = (int64_t)((n_in + 63) / 64) * ((n_out + 63) / 64);
   int64_t s = (1024 + tiles - 1) / tiles, most = (N + 255) / 256;
   if (s > most) s = most;
   if (s >= 8) s &= ~(int64_t)7;
   return (int)(s < 1 ? 1 : s);
+}
+template <class T, int TI, int FACTOR>
+static void dw_launch(DwArgs a, hipStream_t st) {
+  a.tiles_i = (a.Ci + 64 * TI - 1) / (64 * TI);
+  a.tiles_o = (a.Co + 63) / 64;
+  k_linear_dw<T, TI, FACTOR><<<(unsigned)(a.slices * a.tiles_i * a.tiles_o), 256, 0, st>>>(a);
 }
 
 }  // namespace scn
@@ -477,13 +663,12 @@ int scn_dropout(const void *x, int64_t ldx, void *y, int64_t N, int planes, int 
     using T = decltype(t);
     constexpr int Q = Elem<T>::V / 4;
     const bool whole = planes % (4 * Q) == 0;
-    const int items = (planes + 4 * Q - 1) / (4 * Q);
-    int64_t blocks = (N * items + 255) / 256;
-    if (blocks > 4096) blocks = 4096;
-    const int64_t step = blocks * 256;
+    const int items = (planes + 4 * Q - 1) / (4 * Q), rows = items <= 128 ? 256 / items : 1, slabs = items <= 128 ? 1 : (items + 255) / 256;
+    int64_t blocks = (N + rows - 1) / rows, most = 4096 / slabs;
+    if (blocks > most) blocks = most < 1 ? 1 : most;
     auto k = whole ? k_dropout<T, Q, true> : k_dropout<T, Q, false>;
-    k<<<(unsigned)blocks, 256, 0, as_stream(stream)>>>((const T *)x, ldx, (T *)y, N, planes, items, step / items,
-                                                       (int)(step % items), drop_threshold(p), (float)(1.0 / (1.0 - p)), rng);
+    k<<<dim3((unsigned)blocks, slabs), 256, 0, as_stream(stream)>>>((const T *)x, ldx, (T *)y, N, planes, items, rows, drop_threshold(p),
+                                                                  (float)(1.0 / (1.0 - p)), rng);
     SCN_CHECK_LAUNCH();
     return 0;
   });
@@ -519,30 +704,35 @@ int scn_linear_forward(const void *x, int64_t ldx, const void *weight, const voi
   a.M = n_out;
   a.threshold = drop_threshold(p);
   a.leak = (float)leakiness;
-  a.keep_scale = (float)(1.0 / (1.0 - p));
+  a.up = (float)(1.0 / (1.0 - p));
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    if (act == SCN_ACT_SILU) return linear_by_width<T, 0, SCN_ACT_SILU>(a, as_stream(stream));
-    if (act == SCN_ACT_GELU) return linear_by_width<T, 0, SCN_ACT_GELU>(a, as_stream(stream));
-    return linear_by_width<T, 0, SCN_ACT_LEAKY>(a, as_stream(stream));
+    if (act == SCN_ACT_SILU) return linear_forward<T, SCN_ACT_SILU>(a, as_stream(stream));
+    if (act == SCN_ACT_GELU) return linear_forward<T, SCN_ACT_GELU>(a, as_stream(stream));
+    return linear_forward<T, SCN_ACT_LEAKY>(a, as_stream(stream));
   });
 }
 
 int scn_linear_dinput(const void *d_y, int64_t ld_dy, const void *factor, const void *weight, void *d_x, int64_t N, int n_in,
-                      int n_out, int dtype, void *stream) {
+                      int n_out, int act, double leakiness, double p, int dtype, void *stream) {
   if (int e = lin_check(N, n_in, n_out, dtype)) return e;
+  SCN_REQUIRE(p >= 0 && p < 1, "linear: 0 <= p < 1");
   if (N == 0) return 0;
   SCN_REQUIRE(d_y && weight && d_x && ld_dy >= n_out, "linear: pointers");
   LinearArgs a = {};
   a.in = d_y;
   a.ld_in = ld_dy;
-  a.scale = factor;
+  a.factor_in = factor;
+  a.scale = factor_scale(leakiness, p);
   a.weight = weight;
   a.out = d_x;
   a.N = N;
   a.K = n_out;
   a.M = n_in;
-  return by_type(dtype, [&](auto t) { return linear_by_width<decltype(t), 1, SCN_ACT_LEAKY>(a, as_stream(stream)); });
+  return by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    return by_factor<T>(factor, act, [&](auto f) { return linear_by_width<T, 1, decltype(f)::value>(a, as_stream(stream)); });
+  });
 }
 
 size_t scn_linear_dweight_temp_bytes(int64_t N, int n_in, int n_out) {
@@ -550,21 +740,22 @@ size_t scn_linear_dweight_temp_bytes(int64_t N, int n_in, int n_out) {
 }
 
 int scn_linear_dweight(const void *x, int64_t ldx, const void *d_y, int64_t ld_dy, const void *factor, void *d_weight, void *d_bias,
-                       int64_t N, int n_in, int n_out, int dtype, void *temp, size_t temp_bytes, void *stream) {
+                       int64_t N, int n_in, int n_out, int act, double leakiness, double p, int dtype, void *temp,
+                       size_t temp_bytes, void *stream) {
   if (int e = lin_check(N, n_in, n_out, dtype)) return e;
+  SCN_REQUIRE(p >= 0 && p < 1, "linear: 0 <= p < 1");
   SCN_REQUIRE(d_weight && (N == 0 || (x && d_y)) && ldx >= n_in && ld_dy >= n_out, "linear: pointers");
   SCN_REQUIRE(temp && temp_bytes >= scn_linear_dweight_temp_bytes(N, n_in, n_out), "linear: workspace");
   DwArgs a = {};
   a.x = x;
   a.dy = d_y;
-  a.scale = factor;
+  a.factor = factor;
+  a.scale = factor_scale(leakiness, p);
   a.ldx = ldx;
   a.ld_dy = ld_dy;
   a.N = N;
   a.Ci = n_in;
   a.Co = n_out;
-  a.tiles_i = (n_in + 63) / 64;
-  a.tiles_o = (n_out + 63) / 64;
   a.slices = dw_slices(N, n_in, n_out);
   a.slice_rows = ((N + a.slices - 1) / a.slices + 127) / 128 * 128;
   a.slab = (float *)temp;
@@ -573,9 +764,18 @@ int scn_linear_dweight(const void *x, int64_t ldx, const void *d_y, int64_t ld_d
   const int nb = d_bias ? n_out : 0;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    k_linear_dw<T><<<(unsigned)(a.slices * a.tiles_i * a.tiles_o), 256, 0, as_stream(stream)>>>(a);
+    by_factor<T>(factor, act, [&](auto f) {
+      constexpr int FACTOR = decltype(f)::value;
+      if constexpr (dw_wide<T, FACTOR>())
+        if (n_in > 64) {
+          dw_launch<T, 2, FACTOR>(a, as_stream(stream));
+          return 0;
+        }
+      dw_launch<T, 1, FACTOR>(a, as_stream(stream));
+      return 0;
+    });
     SCN_CHECK_LAUNCH();
-    k_linear_dw_join<T><<<(unsigned)((nw + nb + 255) / 256), 256, 0, as_stream(stream)>>>(a.slab, a.slices, nw, nb, (T *)d_weight,
+    k_linear_dw_join<T><<<(unsigned)((nw + nb + 63) / 64), 1024, 0, as_stream(stream)>>>(a.slab, a.slices, nw, nb, (T *)d_weight,
                                                                                          (T *)d_bias);
     SCN_CHECK_LAUNCH();
     return 0;

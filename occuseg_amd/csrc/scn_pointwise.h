@@ -36,46 +36,58 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r) {
 // ACT: SCN_ACT_LEAKY  z > 0 ? z : leak * z      (leak 0 = ReLU, 1 = none)
 //      SCN_ACT_SILU   z / (1 + e^-z)
 //      SCN_ACT_GELU   z Phi(z), Phi the normal distribution function
-// EXACT (float features): expf / erff.  Otherwise the result is rounded to 8 or 11 bits behind this: the hardware's exp2, and
-// Phi from Abramowitz & Stegun, Handbook of Mathematical Functions, 7.1.26 (|error of erf| <= 1.5e-7), which shares its
-// exponential with the slope.
-template <int ACT, bool EXACT>
+// One reciprocal and one exponential of the hardware each (1 ulp; an exponent x is off by |x| 2^-24, where e^x is as small).  The tail
+// 1 - Phi(t), t >= 0, is e^(-t^2 / 2) times a smooth function of t, here a polynomial in s = 1 / (1 + c t) without a constant term,
+// fitted to erfcx(t / sqrt 2) / 2 over t <= 40 by iteratively reweighted least squares.  Largest relative error of z Phi(z) in fp32 over
+// |z| <= 9: 4.5e-7 with nine terms (FINE, float features), 2.9e-6 with seven (16-bit features: 2^-12 at the finest).
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <int ACT, bool FINE>
 __device__ __forceinline__ void act_value_slope(float z, float leak, float &value, float &slope) {
   if (ACT == SCN_ACT_LEAKY) {
     slope = z > 0 ? 1.f : leak;
-    value = z > 0 ? z : z * leak;
+    value = z * slope;
   } else if (ACT == SCN_ACT_SILU) {
-    const float e = EXACT ? expf(-z) : __expf(-z);
-    const float s = EXACT ? 1.f / (1.f + e) : __builtin_amdgcn_rcpf(1.f + e);
+    const float s = __builtin_amdgcn_rcpf(1.f + exp2_hw(z * -1.44269504f));
     value = z * s;
-    slope = s * fmaf(z, 1.f - s, 1.f);
+    slope = fmaf(value, 1.f - s, s);
   } else {
-    float cdf, dens;  // Phi(z), its derivative
-    if (EXACT) {
-      cdf = fmaf(0.5f, erff(z * 0.70710678f), 0.5f);
-      dens = 0.39894228f * expf(-0.5f * z * z);
+    const float e = exp2_hw(z * z * -0.72134752f), t = fabsf(z);
+    float p;
+    if (FINE) {
+      const float s = __builtin_amdgcn_rcpf(fmaf(0.36f, t, 1.f));
+      p = fmaf(s, -0.030251468f, 0.139558294f);
+      p = fmaf(s, p, -0.223676858f);
+      p = fmaf(s, p, 0.107432581f);
+      p = fmaf(s, p, -0.000416137f);
+      p = fmaf(s, p, 0.096045419f);
+      p = fmaf(s, p, 0.124008544f);
+      p = fmaf(s, p, 0.143681972f);
+      p = fmaf(s, p, 0.143617662f) * s;
     } else {
-      const float e = __expf(-0.5f * z * z);
-      const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
-      const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-      const float tail = 0.5f * poly * e;  // 1 - Phi(|z|)
-      cdf = z > 0 ? 1.f - tail : tail;
-      dens = 0.39894228f * e;
+      const float s = __builtin_amdgcn_rcpf(fmaf(0.38f, t, 1.f));
+      p = fmaf(s, 0.048951976f, -0.160032814f);
+      p = fmaf(s, p, 0.114400200f);
+      p = fmaf(s, p, 0.059983662f);
+      p = fmaf(s, p, 0.133793775f);
+      p = fmaf(s, p, 0.151298799f);
+      p = fmaf(s, p, 0.151605686f) * s;
     }
+    const float tail = p * e, cdf = z > 0 ? 1.f - tail : tail;
     value = z * cdf;
-    slope = fmaf(z, dens, cdf);
+    slope = fmaf(z * 0.39894228f, e, cdf);
   }
 }
-template <int ACT, bool EXACT>
+template <int ACT, bool FINE>
 __device__ __forceinline__ float act_value(float z, float leak) {
   float v, s;
-  act_value_slope<ACT, EXACT>(z, leak, v, s);
+  act_value_slope<ACT, FINE>(z, leak, v, s);
   return v;
 }
-template <int ACT, bool EXACT>
+template <int ACT, bool FINE>
 __device__ __forceinline__ float act_slope(float z, float leak) {
   float v, s;
-  act_value_slope<ACT, EXACT>(z, leak, v, s);
+  act_value_slope<ACT, FINE>(z, leak, v, s);
   return s;
 }
 
@@ -93,17 +105,45 @@ __device__ __forceinline__ RngKey rng_key(const int64_t *rng) {
   const uint64_t seed = (uint64_t)rng[0], offset = (uint64_t)rng[1];
   return RngKey{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)offset, (uint32_t)(offset >> 32)};
 }
-__device__ __forceinline__ Words philox(RngKey key, uint32_t quad, uint32_t site) {
-  uint32_t c0 = quad, c1 = site, c2 = key.c2, c3 = key.c3, k0 = key.k0, k1 = key.k1;
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
+// Products of rounds 1 to 3 depend on the plane (P) or on the site (S) alone: c = (quad, site, c2, c3) gives
+//   round 1: quad M0 (P), c2 M1 (uniform)    round 2: f(site) M0 (S), f(quad) M1 (P)    round 3: f(quad) M0 (P), both M1
+// so a thread that keeps its planes makes 16 of the 20 per site, one that keeps both halves 15.
+struct PhiloxPlane {
+  uint32_t c1, c2x, r3lo, r3hi;  // see philox_plane
+};
+struct PhiloxSite {
+  uint32_t hi, lo;
+};
+constexpr uint32_t PH_M0 = 0xD2511F53u, PH_M1 = 0xCD9E8D57u, PH_W0 = 0x9E3779B9u, PH_W1 = 0xBB67AE85u;
+__device__ __forceinline__ PhiloxPlane philox_plane(RngKey k, uint32_t quad) {
+  const uint64_t a1 = (uint64_t)quad * PH_M0, b1 = (uint64_t)k.c2 * PH_M1;
+  // after round 1: (hi(b1) ^ site ^ k0, lo(b1), hi(a1) ^ c3 ^ k1, lo(a1))
+  const uint64_t b2 = (uint64_t)xor3((uint32_t)(a1 >> 32), k.c3, k.k1) * PH_M1;
+  // after round 2: (hi(b2) ^ lo(b1) ^ k0', lo(b2), hi(a2) ^ lo(a1) ^ k1', lo(a2)),  a2 = (hi(b1) ^ site ^ k0) M0
+  const uint64_t a3 = (uint64_t)xor3((uint32_t)(b2 >> 32), (uint32_t)b1, k.k0 + PH_W0) * PH_M0;
+  // round 3 takes c1 = lo(b2) ^ k0'', c2 ^ .. = lo(a1) ^ k1', and a3
+  return PhiloxPlane{(uint32_t)b2 ^ (k.k0 + 2 * PH_W0), (uint32_t)a1 ^ (k.k1 + PH_W1), (uint32_t)a3, (uint32_t)(a3 >> 32) ^ (k.k1 + 2 * PH_W1)};
+}
+__device__ __forceinline__ PhiloxSite philox_site(RngKey k, uint32_t site) {
+  const uint64_t b1 = (uint64_t)k.c2 * PH_M1;
+  const uint64_t a2 = (uint64_t)xor3((uint32_t)(b1 >> 32), site, k.k0) * PH_M0;
+  return PhiloxSite{(uint32_t)(a2 >> 32), (uint32_t)a2};
+}
+__device__ __forceinline__ Words philox(RngKey k, const PhiloxPlane &p, const PhiloxSite &s) {
+  // round 3
+  const uint64_t b3 = (uint64_t)(s.hi ^ p.c2x) * PH_M1;
+  uint32_t c0 = (uint32_t)(b3 >> 32) ^ p.c1, c1 = (uint32_t)b3, c2 = p.r3hi ^ s.lo, c3 = p.r3lo;
+  uint32_t k0 = k.k0 + 3 * PH_W0, k1 = k.k1 + 3 * PH_W1;
 #pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+  for (int r = 3; r < 10; ++r) {
+    const uint64_t a = (uint64_t)c0 * PH_M0, b = (uint64_t)c2 * PH_M1;
+    c0 = xor3((uint32_t)(b >> 32), c1, k0);
     c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c2 = xor3((uint32_t)(a >> 32), c3, k1);
     c3 = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
+    k0 += PH_W0;
+    k1 += PH_W1;
   }
   return Words{{c0, c1, c2, c3}};
 }

@@ -79,10 +79,10 @@ class _FusedNiNFunction(Function):
         out = like_empty(features)
         # what the backward pass needs of activation and mask: their common derivative, one value per output
         wanted = any(ctx.needs_input_grad[:3]) and (p > 0 or activation != "leaky_relu" or leakiness != 1)
-        factor = like_empty(features) if wanted else None
+        factor = torch.empty(0, dtype=SCN.factor_dtype(features), device=features.device) if wanted else None
         macs = SCN.FusedNetworkInNetwork_updateOutput(features, out, weight, bias, residual, activation, leakiness, p, rng, factor)
         counters.add(macs, out.nelement())
-        ctx.has_bias = bias.numel() > 0
+        ctx.has_bias, ctx.args = bias.numel() > 0, (activation, leakiness, p)
         ctx.save_for_backward(features, weight, factor)
         return out
 
@@ -96,7 +96,7 @@ class _FusedNiNFunction(Function):
         grad_weight = like_empty(grad_output) if need_w or need_b else None
         grad_bias = like_empty(grad_output) if need_b else None
         if need_x or need_w or need_b:
-            SCN.FusedNetworkInNetwork_backward(features, grad_input, grad_output, weight, grad_weight, grad_bias, factor)
+            SCN.FusedNetworkInNetwork_backward(features, grad_input, grad_output, weight, grad_weight, grad_bias, *ctx.args, factor)
         return (grad_input, grad_weight if need_w else None, grad_bias, grad_output if need_res else None) + (None,) * 4
 
 

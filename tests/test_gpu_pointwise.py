@@ -523,7 +523,7 @@ def test_refusals(gpu):
                                                              1e-4, 2, "silu", 1),
                  lambda: SCN.GroupNormalization_updateOutput(torch.zeros(4, 8192, device=gpu), x.new_empty(0), x.new_empty(0),
                                                              torch.tensor([0, 4], device=gpu), None, None, 1e-4, 2, "silu", 1),
-                 lambda: SCN.FusedNetworkInNetwork_backward(x, None, x, torch.zeros(8, 4, device=gpu), None, None)):
+                 lambda: SCN.FusedNetworkInNetwork_backward(x, None, x, torch.zeros(8, 4, device=gpu), None, None, "silu", 1, 0.0)):
         with pytest.raises(RuntimeError):
             call()
     xg = x.clone().requires_grad_(True)
