@@ -7,7 +7,7 @@
 // done while it is in registers.
 //
 // Products: v_mfma 16x16, the WEIGHT as the A operand and the sites as B: the four results of a lane are then four consecutive
-// planes of one site -- one random-number counter, one wide store -- and 16 sites x 64 bytes a store instruction.  The order of the
+// planes of one site.  The order of the
 // reduction is free as long as both operands agree: a lane's 16 bytes of a row, loaded straight from global memory, ARE its B
 // operands (one 16x16x32 of 16-bit types, four 16x16x4 of fp32).  The weights are laid out in LDS in the order of the A operands.
 #include "scn_pointwise.h"
@@ -158,11 +158,7 @@ __device__ __forceinline__ float epilogue(float z, bool keep, float res, const L
 
 constexpr int LIN_ROWS = 128;  // rows of a workgroup's tile: 4 waves x 2 x 16
 
-// the plane of A row i of column tile t: 16 bytes of consecutive planes per lane (16-bit types: of two tiles together)
-template <class T>
-__device__ __forceinline__ int tile_col(int t, int i) {
-  return sizeof(T) == 4 ? 16 * t + i : 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3);
-}
+constexpr int lin_piece(int nt) { return nt < 4 ? 16 * nt : 64; }  // planes of a tile that go through LDS together
 
 // MODE 0: forward with the epilogue, X its activation.  MODE 1: dx, X how the factors are stored.
 // A workgroup holds the weights of NT x 16 output planes in LDS -- all of K, once, if they fit (then its waves walk their rows
@@ -175,7 +171,9 @@ __global__ void __launch_bounds__(256, 3) k_linear(LinearArgs a) {
   extern __shared__ char smem[];
   F *wl = (F *)smem;  // [k-group of the chunk][tile][lane]
   float *bl = (float *)(wl + (size_t)NT * a.chunk_groups * 64);
-  const int lane = lane_id(), wave = threadIdx.x >> 6, li = lane & 15, lq = lane >> 4;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lq = lane >> 4;
+  constexpr int PC = lin_piece(NT), PITCH = PC + 4, LPR = PC / V;
+  float *sw = bl + NT * 16 + wave * 16 * PITCH;
   // the column blocks of one row block run on one XCD (workgroup ids go round the 8 of them): its rows come from that L2 once
   const int per = a.row_blocks * a.col_blocks, id = blockIdx.x;
   int cb, rb;
@@ -221,7 +219,7 @@ __global__ void __launch_bounds__(256, 3) k_linear(LinearArgs a) {
 #pragma unroll STAGE_UNROLL
         for (int e = threadIdx.x; e < NT * ng * 64; e += 256) {
           const int l = e & 63, t = (e >> 6) % NT, g = (e >> 6) / NT;
-          const int m = m0 + tile_col<T>(t, l & 15), k = (g0 + g) * KG + (l >> 4) * V;
+          const int m = m0 + 16 * t + (l & 15), k = (g0 + g) * KG + (l >> 4) * V;
           Pack<T, V> v;
           if (MODE == 1) v = load_some<T, V>(wt + (int64_t)m * a.K + k, m < a.M ? a.K - k : 0);
           else
@@ -273,47 +271,65 @@ __global__ void __launch_bounds__(256, 3) k_linear(LinearArgs a) {
       if (g < nf) batch(std::integral_constant<int, 1>(), std::true_type(), g++);
       if (g < ng) batch(std::integral_constant<int, 1>(), std::false_type(), g);
     }
-    constexpr int TP = V / 4;  // tiles per 16-byte store
-    PhiloxSite site[2] = {};
-    if (MODE == 0 && a.threshold) {
-      site[0] = philox_site(key, (uint32_t)row0);
-      site[1] = philox_site(key, (uint32_t)row0 + 16);
-    }
+    // Results go through LDS, 16 sites x PC planes of a wave at a time: a lane then has 16 bytes of a row and its neighbours the bytes
+    // beside them, 4 rows x 256 bytes (fp32) or 8 rows x 128 an instruction.  Stored from where the product leaves them they are
+    // 16 pieces of 64 bytes, half a cache line each: 226 MB of the wide layer took 149 us that way, of 43 at the copy rate.
 #pragma unroll
-    for (int t = 0; t < NT; t += TP) {
-      const int cl = tile_col<T>(t, 4 * lq), m = m0 + cl;
-      if (m >= a.M) continue;
-      PhiloxPlane plane[TP] = {};
-      if (MODE == 0 && a.threshold)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int q = 0; q < TP; ++q) plane[q] = philox_plane(key, (uint32_t)((m >> 2) + q));
+      for (int pc = 0; pc < NT * 16; pc += PC) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int64_t row = row0 + 16 * u;
-        if (row >= a.N) continue;
-        Pack<T, V> y;
-        if constexpr (MODE == 1) {
+        for (int t = pc / 16; t < (pc + PC) / 16; ++t) *(floatx4 *)(sw + li * PITCH + 16 * t + 4 * lq - pc) = acc[u][t];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int cl = pc + lane % LPR * V, m = m0 + cl;
+        PhiloxPlane plane[V / 4] = {};
+        float bias[V];
+        if (MODE == 0) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) y.v[j] = (T)acc[u][t + j / 4][j & 3];
-        } else {
-          Pack<T, V> res;
-          Pack<Q, V> f;
-          if (a.residual) res = load_some<T, V>((const T *)a.residual + row * a.ld_res + m, a.M - m);
+          for (int j = 0; j < V; ++j) bias[j] = bl[cl + j];
+          if (a.threshold)
 #pragma unroll
-          for (int q = 0; q < TP; ++q) {
-            Words w;
-            if (a.threshold) w = philox(key, plane[q], site[u]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              y.v[4 * q + j] = (T)epilogue<T, X>(acc[u][t + q][j] + bl[cl + 4 * q + j], !a.threshold || w.w[j] >= a.threshold,
-                                                 a.residual ? (float)res.v[4 * q + j] : 0.f, a, f.v[4 * q + j]);
-          }
-          if (a.factor) store_some<Q, V>((Q *)a.factor + row * a.M + m, f, a.M - m);
+            for (int q = 0; q < V / 4; ++q) plane[q] = philox_plane(key, (uint32_t)((m >> 2) + q));
         }
-        store_some<T, V>((T *)a.out + row * a.M + m, y, a.M - m);
+#pragma unroll
+        for (int it = 0; it < 16; it += 64 / LPR) {
+          const int r = it + lane / LPR;
+          float z[V];
+#pragma unroll
+          for (int j = 0; j < V; j += 4) {
+            const floatx4 v = *(const floatx4 *)(sw + r * PITCH + cl - pc + j);
+            z[j] = v[0], z[j + 1] = v[1], z[j + 2] = v[2], z[j + 3] = v[3];
+          }
+          const int64_t row = tile * LIN_ROWS + wave * 32 + 16 * u + r;
+          if (row >= a.N || m >= a.M) continue;
+          Pack<T, V> y;
+          if constexpr (MODE == 1) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) y.v[j] = (T)z[j];
+          } else {
+            Pack<T, V> res;
+            Pack<Q, V> f;
+            if (a.residual) res = load_some<T, V>((const T *)a.residual + row * a.ld_res + m, a.M - m);
+            PhiloxSite site = {};
+            if (a.threshold) site = philox_site(key, (uint32_t)row);
+#pragma unroll
+            for (int q = 0; q < V / 4; ++q) {
+              Words w;
+              if (a.threshold) w = philox(key, plane[q], site);
+#pragma unroll
+              for (int j = 4 * q; j < 4 * q + 4; ++j)
+                y.v[j] = (T)epilogue<T, X>(z[j] + bias[j], !a.threshold || w.w[j & 3] >= a.threshold, a.residual ? (float)res.v[j] : 0.f, a,
+                                           f.v[j]);
+            }
+            if (a.factor) store_some<Q, V>((Q *)a.factor + row * a.M + m, f, a.M - m);
+          }
+          store_some<T, V>((T *)a.out + row * a.M + m, y, a.M - m);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_sched_barrier(0);  // (one piece at a time: all of them interleaved do not fit the registers)
       }
-      __builtin_amdgcn_sched_barrier(0);  // (one tile's epilogue at a time: all of them interleaved do not fit the registers)
-    }
   }
 }
 
@@ -586,14 +602,15 @@ static int linear_launch(LinearArgs a, hipStream_t st) {
   constexpr int KG = 4 * Elem<T>::V, group_bytes = NT * 64 * 16;
   a.groups = (a.K + KG - 1) / KG;
   a.chunk_groups = a.groups;
-  if (a.groups * group_bytes > 61440) a.chunk_groups = 32768 / group_bytes;
+  const size_t rest = NT * 16 * 4 + 4 * 16 * (lin_piece(NT) + 4) * 4;  // bias, results
+  if (a.groups * group_bytes + rest > 65536) a.chunk_groups = 32768 / group_bytes;
   a.col_blocks = (a.M + NT * 16 - 1) / (NT * 16);
   const int64_t tiles = (a.N + LIN_ROWS - 1) / LIN_ROWS;
   int64_t rows = 1024 / a.col_blocks;
   if (rows < 1) rows = 1;
   if (a.groups > a.chunk_groups || rows > tiles) rows = tiles;  // (weights that do not stay: one tile a workgroup)
   a.row_blocks = (int)rows;
-  const size_t lds = (size_t)a.chunk_groups * group_bytes + NT * 16 * 4;
+  const size_t lds = (size_t)a.chunk_groups * group_bytes + rest;
   k_linear<T, NT, MODE, X><<<(unsigned)(rows * a.col_blocks), 256, lds, st>>>(a);
   SCN_CHECK_LAUNCH();
   return 0;
