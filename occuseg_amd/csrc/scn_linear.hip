@@ -145,15 +145,23 @@ struct LinearArgs {
   FactorScale scale;
 };
 
-// one output's activation, mask, residual; a kept or dropped element's factor
-template <class T, int ACT>
-__device__ __forceinline__ float epilogue(float z, bool keep, float res, const LinearArgs &a, typename FactorOf<T>::type &factor) {
-  float value, slope;
-  act_value_slope<ACT, sizeof(T) == 4>(z, a.leak, value, slope);
-  if constexpr (sizeof(T) == 4) factor = keep ? slope * a.up : 0.f;
-  else if (ACT == SCN_ACT_LEAKY) factor = keep ? (z > 0 ? 2 : 1) : 0;
-  else factor = !keep ? 0 : slope == slope ? (int16_t)(int)rintf(slope * 16384.f) : -32768;
-  return (keep ? value * a.up : 0.f) + res;
+constexpr int ACT_NONE = 3;  // SCN_ACT_LEAKY with slope 1
+
+// one output's activation and mask, and its factor
+template <class T, int ACT, bool DROP>
+__device__ __forceinline__ float activated(float z, bool keep, const LinearArgs &a, typename FactorOf<T>::type &factor) {
+  float value = z, slope = 1.f;
+  if constexpr (ACT != ACT_NONE) act_value_slope<ACT, sizeof(T) == 4>(z, a.leak, value, slope);
+  if constexpr (DROP) value = keep ? value * a.up : 0.f;
+  if constexpr (sizeof(T) == 4) {
+    factor = DROP ? (keep ? slope * a.up : 0.f) : slope;
+  } else {
+    if constexpr (ACT == ACT_NONE) factor = 2;
+    else if constexpr (ACT == SCN_ACT_LEAKY) factor = z > 0 ? 2 : 1;
+    else factor = slope == slope ? (int16_t)(int)rintf(slope * 16384.f) : -32768;
+    if (DROP && !keep) factor = 0;
+  }
+  return value;
 }
 
 constexpr int LIN_ROWS = 128;  // rows of a workgroup's tile: 4 waves x 2 x 16
@@ -161,18 +169,22 @@ constexpr int LIN_ROWS = 128;  // rows of a workgroup's tile: 4 waves x 2 x 16
 constexpr int lin_piece(int nt) { return nt < 4 ? 16 * nt : 64; }  // planes of a tile that go through LDS together
 
 // MODE 0: forward with the epilogue, X its activation.  MODE 1: dx, X how the factors are stored.
-// A workgroup holds the weights of NT x 16 output planes in LDS -- all of K, once, if they fit (then its waves walk their rows
-// without a barrier), else `chunk_groups` at a time -- and walks the row tiles row_block, row_block + row_blocks, ...
+// A workgroup holds the weights of NT x 16 output planes in LDS -- all of K, once, if they fit: then its waves walk 32-row tiles of
+// their own without a barrier -- else `chunk_groups` at a time, and its waves keep together.
+// Beside fp32 MFMAs a vector instruction costs 8 or more of the matrix pipe's cycles, and the epilogue alone fills half the time of
+// a 16-bit layer: addresses are a scalar base and one 32-bit offset a lane for all tiles, the bias is what the accumulators start
+// from, and the epilogue is compiled for each activation, with and without dropout and factors.
 template <class T, int NT, int MODE, int X>
-__global__ void __launch_bounds__(256, 3) k_linear(LinearArgs a) {
+__global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
   constexpr int V = Elem<T>::V, KG = 4 * V, STAGE_UNROLL = MODE == 0 ? 4 : 1;
+  constexpr int PC = lin_piece(NT), PITCH = PC + 4, LPR = PC / V, RPI = 64 / LPR;  // planes, lanes a row, rows an instruction of a piece
+  constexpr bool FACTORS = MODE == 1 && X != FACTOR_NONE;
   using F = typename Frag<T>::type;
   using Q = typename FactorOf<T>::type;
   extern __shared__ char smem[];
   F *wl = (F *)smem;  // [k-group of the chunk][tile][lane]
   float *bl = (float *)(wl + (size_t)NT * a.chunk_groups * 64);
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lq = lane >> 4;
-  constexpr int PC = lin_piece(NT), PITCH = PC + 4, LPR = PC / V;
   float *sw = bl + NT * 16 + wave * 16 * PITCH;
   // the column blocks of one row block run on one XCD (workgroup ids go round the 8 of them): its rows come from that L2 once
   const int per = a.row_blocks * a.col_blocks, id = blockIdx.x;
@@ -188,148 +200,185 @@ __global__ void __launch_bounds__(256, 3) k_linear(LinearArgs a) {
   const int m0 = cb * NT * 16;
   const T *in = (const T *)a.in, *wt = (const T *)a.weight;
   const Q *fi = (const Q *)a.factor_in;
-  if (MODE == 0 && threadIdx.x < NT * 16) {
+  if (threadIdx.x < NT * 16) {
     const int m = m0 + threadIdx.x;
-    bl[threadIdx.x] = a.bias && m < a.M ? (float)((const T *)a.bias)[m] : 0.f;
+    bl[threadIdx.x] = MODE == 0 && a.bias && m < a.M ? (float)((const T *)a.bias)[m] : 0.f;
   }
   RngKey key = {};
   if (MODE == 0 && a.threshold) key = rng_key(a.rng);
   const int full = a.K / KG;  // k-groups that lie inside the rows
-  bool staged = false;
-  const int64_t tiles = (a.N + LIN_ROWS - 1) / LIN_ROWS;
-  for (int64_t tile = rb; tile < tiles; tile += a.row_blocks) {
+  const bool stay = a.groups <= a.chunk_groups;
+  const int tiles = (int)(stay ? (a.N + 31) / 32 : (a.N + LIN_ROWS - 1) / LIN_ROWS * 4);
+
+  auto stage = [&](int g0, int ng) __attribute__((always_inline)) {
+#pragma unroll STAGE_UNROLL
+    for (int e = threadIdx.x; e < NT * ng * 64; e += 256) {
+      const int l = e & 63, t = (e >> 6) % NT, g = (e >> 6) / NT;
+      const int m = m0 + 16 * t + (l & 15), k = (g0 + g) * KG + (l >> 4) * V;
+      Pack<T, V> v;
+      if (MODE == 1) v = load_some<T, V>(wt + (int64_t)m * a.K + k, m < a.M ? a.K - k : 0);
+      else
+#pragma unroll
+        for (int j = 0; j < V; ++j) v.v[j] = m < a.M && k + j < a.K ? wt[(int64_t)(k + j) * a.M + m] : (T)0.f;
+      __builtin_memcpy(&wl[e], &v, 16);
+    }
+  };
+  if (stay) stage(0, a.groups);
+  __syncthreads();
+
+  // a piece of results: 16 sites x PC planes from LDS, this lane's V planes of every RPI-th of them
+  auto finish = [&](auto drop, auto fac, int64_t row0, int pc) __attribute__((always_inline)) {
+    constexpr bool DROP = decltype(drop)::value, FAC = decltype(fac)::value;
+    const int r0 = lane / LPR, c = lane % LPR * V, m = m0 + pc + c, left = a.M - m;
+    if (left <= 0) return;
+    const int rows = (int)min((int64_t)16, a.N - row0);
+    // (scalar bases, 32-bit offsets)
+    T *out = (T *)a.out + row0 * a.M + m0 + pc;
+    Q *fo = (Q *)a.factor + row0 * a.M + m0 + pc;
+    const T *res = (const T *)a.residual + row0 * a.ld_res + m0 + pc;
+    const unsigned o0 = (unsigned)(r0 * a.M + c), res0 = (unsigned)(r0 * (int)a.ld_res + c);
+    PhiloxPlane plane[V / 4];
+    if constexpr (DROP)
+#pragma unroll
+      for (int q = 0; q < V / 4; ++q) plane[q] = philox_plane(key, (uint32_t)((m >> 2) + q));
+#pragma unroll
+    for (int it = 0; it < 16; it += RPI) {
+      if (it + r0 >= rows) break;
+      float z[V];
+#pragma unroll
+      for (int j = 0; j < V; j += 4) {
+        const floatx4 v = *(const floatx4 *)(sw + (it + r0) * PITCH + c + j);
+        z[j] = v[0], z[j + 1] = v[1], z[j + 2] = v[2], z[j + 3] = v[3];
+      }
+      Pack<T, V> y;
+      if constexpr (MODE == 1) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) y.v[j] = (T)z[j];
+      } else {
+        Pack<Q, V> f;
+        PhiloxSite site;
+        if constexpr (DROP) site = philox_site(key, (uint32_t)(row0 + it) + r0);
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+          Words w;
+          if constexpr (DROP) w = philox(key, plane[q], site);
+#pragma unroll
+          for (int j = 4 * q; j < 4 * q + 4; ++j) z[j] = activated<T, X, DROP>(z[j], !DROP || w.w[j & 3] >= a.threshold, a, f.v[j]);
+        }
+        if (a.residual) {
+          const Pack<T, V> rv = load_some<T, V>(res + it * a.ld_res + res0, left);
+#pragma unroll
+          for (int j = 0; j < V; ++j) z[j] += (float)rv.v[j];
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) y.v[j] = (T)z[j];
+        if constexpr (FAC) store_some<Q, V>(fo + (int64_t)it * a.M + o0, f, left);
+      }
+      store_some<T, V>(out + (int64_t)it * a.M + o0, y, left);
+    }
+  };
+
+  for (int tile = rb * 4 + wave; tile < tiles; tile += a.row_blocks * 4) {
+    const int64_t row0 = (int64_t)tile * 32;
+    // (rows behind the last are read as the last and not written; of tiles behind the last, too)
+    const int64_t base = min(row0, a.N - 1);
+    const int last = (int)min((int64_t)31, a.N - 1 - base);
+    const T *p = in + base * a.ld_in;
+    const Q *pf = fi + base * a.K;
+    unsigned op[2], of[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = min(li + 16 * u, last);
+      op[u] = (unsigned)(r * (int)a.ld_in + lq * V);
+      of[u] = (unsigned)(r * a.K + lq * V);
+    }
     floatx4 acc[2][NT];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int t = 0; t < NT; ++t) acc[0][t] = acc[1][t] = *(const floatx4 *)(bl + 16 * t + 4 * lq);
+
+    // G k-groups: their rows are requested together (a row's two halves of a cache line one behind the other), then multiplied
+    auto batch = [&](auto count, auto whole, int g, const F *wg) __attribute__((always_inline)) {
+      constexpr int G = decltype(count)::value;
+      constexpr bool WHOLE = decltype(whole)::value;
+      Pack<T, V> v[G][2];
+      Pack<Q, V> f[G][2];
+      const T *pk = p + g * KG;
+      const Q *pfk = pf + g * KG;
+      const int left = a.K - g * KG - lq * V;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) acc[u][t] = floatx4{0.f, 0.f, 0.f, 0.f};
-    const int64_t row0 = tile * LIN_ROWS + wave * 32 + li;
-    // (rows behind the last are read as the last and not written)
-    const int64_t rr[2] = {min(row0, a.N - 1), min(row0 + 16, a.N - 1)};
-    const T *p[2] = {in + rr[0] * a.ld_in + lq * V, in + rr[1] * a.ld_in + lq * V};
-    const Q *pf[2] = {nullptr, nullptr};
-    if (MODE == 1 && X != FACTOR_NONE) {
-      pf[0] = fi + rr[0] * a.K + lq * V;
-      pf[1] = fi + rr[1] * a.K + lq * V;
-    }
-    for (int g0 = 0; g0 < a.groups; g0 += a.chunk_groups) {
-      const int ng = min(a.chunk_groups, a.groups - g0);
-      if (!staged || a.groups > a.chunk_groups) {
-        __syncthreads();
-#pragma unroll STAGE_UNROLL
-        for (int e = threadIdx.x; e < NT * ng * 64; e += 256) {
-          const int l = e & 63, t = (e >> 6) % NT, g = (e >> 6) / NT;
-          const int m = m0 + 16 * t + (l & 15), k = (g0 + g) * KG + (l >> 4) * V;
-          Pack<T, V> v;
-          if (MODE == 1) v = load_some<T, V>(wt + (int64_t)m * a.K + k, m < a.M ? a.K - k : 0);
-          else
-#pragma unroll
-            for (int j = 0; j < V; ++j) v.v[j] = m < a.M && k + j < a.K ? wt[(int64_t)(k + j) * a.M + m] : (T)0.f;
-          __builtin_memcpy(&wl[e], &v, 16);
-        }
-        __syncthreads();
-        staged = true;
-      }
-      // G k-groups: their rows are requested together, then multiplied
-      auto batch = [&](auto count, auto whole, int g) __attribute__((always_inline)) {
-        constexpr int G = decltype(count)::value;
-        constexpr bool WHOLE = decltype(whole)::value;
-        Pack<T, V> v[G][2];
-        Pack<Q, V> f[G][2];
-#pragma unroll
-        for (int i = 0; i < G; ++i)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int k = (g0 + g + i) * KG, left = a.K - k - lq * V;
-            v[i][u] = WHOLE ? load_pack<T, V>(p[u] + k) : load_some<T, V>(p[u] + k, left);
-            if constexpr (MODE == 1 && X != FACTOR_NONE) f[i][u] = WHOLE ? load_pack<Q, V>(pf[u] + k) : load_some<Q, V>(pf[u] + k, left);
-          }
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-          F b[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            if constexpr (MODE == 1 && X != FACTOR_NONE)
-#pragma unroll
-              for (int j = 0; j < V; ++j) v[i][u].v[j] = (T)((float)v[i][u].v[j] * factor_value<X>(f[i][u].v[j], a.scale));
-            __builtin_memcpy(&b[u], &v[i][u], 16);
-          }
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const F w = wl[((g + i) * NT + t) * 64 + lane];
-            acc[0][t] = mma(w, b[0], acc[0][t]);
-            acc[1][t] = mma(w, b[1], acc[1][t]);
-          }
-          if (NT == 8) __builtin_amdgcn_sched_barrier(0);  // (one k-group's weights in registers at a time)
+          v[i][u] = WHOLE ? load_pack<T, V>(pk + i * KG + op[u]) : load_some<T, V>(pk + i * KG + op[u], left - i * KG);
+          if constexpr (FACTORS) f[i][u] = WHOLE ? load_pack<Q, V>(pfk + i * KG + of[u]) : load_some<Q, V>(pfk + i * KG + of[u], left - i * KG);
         }
-      };
-      const int nf = min(ng, full - g0);
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        F b[2], w[NT];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if constexpr (FACTORS)
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[i][u].v[j] = (T)((float)v[i][u].v[j] * factor_value<X>(f[i][u].v[j], a.scale));
+          __builtin_memcpy(&b[u], &v[i][u], 16);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) w[t] = wg[(i * NT + t) * 64];
+        if constexpr (sizeof(T) == 4) {  // (no product waits for the one in front of it)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[t][j], b[u][j], acc[u][t], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) acc[u][t] = mma(w[t], b[u], acc[u][t]);
+        }
+        if (NT == 8) __builtin_amdgcn_sched_barrier(0);  // (one k-group's weights in registers at a time)
+      }
+    };
+    for (int g0 = 0; g0 < a.groups; g0 += a.chunk_groups) {
+      const int ng = min(a.chunk_groups, a.groups - g0), nf = min(ng, full - g0);
+      if (!stay) {
+        __syncthreads();
+        stage(g0, ng);
+        __syncthreads();
+      }
+      const F *wg = wl + lane;
       int g = 0;
-      if (NT < 8)
-        for (; g + 4 <= nf; g += 4) batch(std::integral_constant<int, 4>(), std::true_type(), g);
-      for (; g + 2 <= nf; g += 2) batch(std::integral_constant<int, 2>(), std::true_type(), g);
-      if (g < nf) batch(std::integral_constant<int, 1>(), std::true_type(), g++);
-      if (g < ng) batch(std::integral_constant<int, 1>(), std::false_type(), g);
+      if (NT < 8 && !(FACTORS && sizeof(T) == 2))
+        for (; g + 4 <= nf; g += 4, wg += 4 * NT * 64) batch(std::integral_constant<int, 4>(), std::true_type(), g0 + g, wg);
+      for (; g + 2 <= nf; g += 2, wg += 2 * NT * 64) batch(std::integral_constant<int, 2>(), std::true_type(), g0 + g, wg);
+      for (; g < nf; ++g, wg += NT * 64) batch(std::integral_constant<int, 1>(), std::true_type(), g0 + g, wg);
+      if (g < ng) batch(std::integral_constant<int, 1>(), std::false_type(), g0 + g, wg);
     }
     // Results go through LDS, 16 sites x PC planes of a wave at a time: a lane then has 16 bytes of a row and its neighbours the bytes
     // beside them, 4 rows x 256 bytes (fp32) or 8 rows x 128 an instruction.  Stored from where the product leaves them they are
     // 16 pieces of 64 bytes, half a cache line each: 226 MB of the wide layer took 149 us that way, of 43 at the copy rate.
+#pragma unroll 1
+    for (int piece = 0; piece < 2 * NT * 16 / PC; ++piece) {
+      constexpr int PPU = NT * 16 / PC;  // pieces of 16 rows
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int k = 0; k < 2 * PPU; ++k)
+        if (k == piece) {
 #pragma unroll
-      for (int pc = 0; pc < NT * 16; pc += PC) {
-#pragma unroll
-        for (int t = pc / 16; t < (pc + PC) / 16; ++t) *(floatx4 *)(sw + li * PITCH + 16 * t + 4 * lq - pc) = acc[u][t];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const int cl = pc + lane % LPR * V, m = m0 + cl;
-        PhiloxPlane plane[V / 4] = {};
-        float bias[V];
-        if (MODE == 0) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) bias[j] = bl[cl + j];
-          if (a.threshold)
-#pragma unroll
-            for (int q = 0; q < V / 4; ++q) plane[q] = philox_plane(key, (uint32_t)((m >> 2) + q));
+          for (int t = 0; t < PC / 16; ++t) *(floatx4 *)(sw + li * PITCH + 16 * t + 4 * lq) = acc[k / PPU][k % PPU * (PC / 16) + t];
         }
-#pragma unroll
-        for (int it = 0; it < 16; it += 64 / LPR) {
-          const int r = it + lane / LPR;
-          float z[V];
-#pragma unroll
-          for (int j = 0; j < V; j += 4) {
-            const floatx4 v = *(const floatx4 *)(sw + r * PITCH + cl - pc + j);
-            z[j] = v[0], z[j + 1] = v[1], z[j + 2] = v[2], z[j + 3] = v[3];
-          }
-          const int64_t row = tile * LIN_ROWS + wave * 32 + 16 * u + r;
-          if (row >= a.N || m >= a.M) continue;
-          Pack<T, V> y;
-          if constexpr (MODE == 1) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) y.v[j] = (T)z[j];
-          } else {
-            Pack<T, V> res;
-            Pack<Q, V> f;
-            if (a.residual) res = load_some<T, V>((const T *)a.residual + row * a.ld_res + m, a.M - m);
-            PhiloxSite site = {};
-            if (a.threshold) site = philox_site(key, (uint32_t)row);
-#pragma unroll
-            for (int q = 0; q < V / 4; ++q) {
-              Words w;
-              if (a.threshold) w = philox(key, plane[q], site);
-#pragma unroll
-              for (int j = 4 * q; j < 4 * q + 4; ++j)
-                y.v[j] = (T)epilogue<T, X>(z[j] + bias[j], !a.threshold || w.w[j & 3] >= a.threshold, a.residual ? (float)res.v[j] : 0.f, a,
-                                           f.v[j]);
-            }
-            if (a.factor) store_some<Q, V>((Q *)a.factor + row * a.M + m, f, a.M - m);
-          }
-          store_some<T, V>((T *)a.out + row * a.M + m, y, a.M - m);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_sched_barrier(0);  // (one piece at a time: all of them interleaved do not fit the registers)
-      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      const int64_t r = row0 + piece / PPU * 16;
+      const int pc = piece % PPU * PC;
+      if (MODE == 1) finish(std::false_type(), std::false_type(), r, pc);
+      else if (a.threshold)
+        a.factor ? finish(std::true_type(), std::true_type(), r, pc) : finish(std::true_type(), std::false_type(), r, pc);
+      else
+        a.factor ? finish(std::false_type(), std::true_type(), r, pc) : finish(std::false_type(), std::false_type(), r, pc);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
   }
 }
 
@@ -382,7 +431,8 @@ __global__ void __launch_bounds__(1024) k_linear_few(LinearArgs a) {
     keep = ((mo & 2) ? (mo & 1) ? w.w[3] : w.w[2] : (mo & 1) ? w.w[1] : w.w[0]) >= a.threshold;
   }
   typename FactorOf<T>::type f;
-  const float y = epilogue<T, ACT>(z, keep, a.residual ? (float)((const T *)a.residual)[row * a.ld_res + mo] : 0.f, a, f);
+  float y = activated<T, ACT, true>(z, keep, a, f);
+  if (a.residual) y += (float)((const T *)a.residual)[row * a.ld_res + mo];
   ((T *)a.out)[(int64_t)row * a.M + mo] = (T)y;
   if (a.factor) ((typename FactorOf<T>::type *)a.factor)[(int64_t)row * a.M + mo] = f;
 }
@@ -606,11 +656,14 @@ static int linear_launch(LinearArgs a, hipStream_t st) {
   if (a.groups * group_bytes + rest > 65536) a.chunk_groups = 32768 / group_bytes;
   a.col_blocks = (a.M + NT * 16 - 1) / (NT * 16);
   const int64_t tiles = (a.N + LIN_ROWS - 1) / LIN_ROWS;
-  int64_t rows = 1024 / a.col_blocks;
-  if (rows < 1) rows = 1;
-  if (a.groups > a.chunk_groups || rows > tiles) rows = tiles;  // (weights that do not stay: one tile a workgroup)
-  a.row_blocks = (int)rows;
   const size_t lds = (size_t)a.chunk_groups * group_bytes + rest;
+  // as many workgroups as the CUs hold, a multiple of the XCDs; weights that do not stay: one tile a workgroup
+  int64_t fit = 163840 / (int64_t)lds;
+  if (fit > (NT == 8 ? 3 : 4)) fit = NT == 8 ? 3 : 4;
+  int64_t rows = 256 * fit / a.col_blocks / 8 * 8;
+  if (rows < 8) rows = 8;
+  if (a.groups > a.chunk_groups || rows > tiles) rows = tiles;
+  a.row_blocks = (int)rows;
   k_linear<T, NT, MODE, X><<<(unsigned)(rows * a.col_blocks), 256, lds, st>>>(a);
   SCN_CHECK_LAUNCH();
   return 0;
@@ -726,6 +779,7 @@ int scn_linear_forward(const void *x, int64_t ldx, const void *weight, const voi
     using T = decltype(t);
     if (act == SCN_ACT_SILU) return linear_forward<T, SCN_ACT_SILU>(a, as_stream(stream));
     if (act == SCN_ACT_GELU) return linear_forward<T, SCN_ACT_GELU>(a, as_stream(stream));
+    if (a.leak == 1.f) return linear_forward<T, ACT_NONE>(a, as_stream(stream));
     return linear_forward<T, SCN_ACT_LEAKY>(a, as_stream(stream));
   });
 }
