@@ -2065,9 +2065,12 @@ def FusedNetworkInNetwork_updateOutput(input_features, output_features, weight, 
             if factor.dtype != factor_dtype(x) or factor.device != x.device:
                 raise RuntimeError("occuseg_amd.SCN.%s: factor must be %s" % (what, factor_dtype(x)))
             factor.resize_(N, Co)
+        lib = _lib_()
+        tb = lib.scn_linear_forward_temp_bytes(N, Ci, Co, code)
+        temp = torch.empty(tb, dtype=torch.uint8, device=x.device) if tb else None
         ev = _prof_begin()
-        check(_lib_().scn_linear_forward(ptr(x), ld, ptr(weight.contiguous()), ptr(bias), ptr(res), ld_res, ptr(output_features),
-                                         ptr(factor), N, Ci, Co, act, float(leakiness), p, ptr(rng), code, stream()))
+        check(lib.scn_linear_forward(ptr(x), ld, ptr(weight.contiguous()), ptr(bias), ptr(res), ld_res, ptr(output_features),
+                                         ptr(factor), N, Ci, Co, act, float(leakiness), p, ptr(rng), code, ptr(temp), tb, stream()))
         _prof_end(ev, "linear_fwd", 2.0 * N * Ci * Co,
                   float(x.element_size()) * (N * (Ci + Co * (1 + (res is not None) + (factor is not None))) + Ci * Co), (N, Ci, Co))
     return float(N) * Ci * Co

@@ -83,7 +83,8 @@ SIGNATURES = {
     "scn_dropout": (c_int, [_P, c_int64, _P, c_int64, c_int, c_int, c_double, _P, _P]),
     "scn_rng_take": (c_int, [_P, _P, _P]),
     "scn_linear_forward": (c_int, [_P, c_int64, _P, _P, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int, c_double, c_double, _P,
-                                   c_int, _P]),
+                                   c_int, _P, c_size_t, _P]),
+    "scn_linear_forward_temp_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
     "scn_linear_dinput": (c_int, [_P, c_int64, _P, _P, _P, c_int64, c_int, c_int, c_int, c_double, c_double, c_int, _P]),
     "scn_linear_dweight_temp_bytes": (c_size_t, [c_int64, c_int, c_int]),
     "scn_linear_dweight": (c_int, [_P, c_int64, _P, c_int64, _P, _P, _P, c_int64, c_int, c_int, c_int, c_double, c_double, c_int, _P,

@@ -131,7 +131,8 @@ __device__ __forceinline__ float factor_value(Q q, const FactorScale &s) {
 struct LinearArgs {
   const void *in, *factor_in;  // rows [N, K] at ld_in elements; MODE 1: times the factors [N, K]
   int64_t ld_in;
-  const void *weight;  // MODE 0: [K, M], MODE 1: [M, K]
+  const void *weight;  // MODE 0: [K, M], MODE 1 and `transposed`: [M, K]
+  int transposed;
   const void *bias, *residual;
   int64_t ld_res;
   void *out, *factor;
@@ -176,7 +177,7 @@ constexpr int lin_piece(int nt) { return nt < 4 ? 16 * nt : 64; }  // planes of 
 // from, and the epilogue is compiled for each activation, with and without dropout and factors.
 template <class T, int NT, int MODE, int X>
 __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
-  constexpr int V = Elem<T>::V, KG = 4 * V, STAGE_UNROLL = MODE == 0 ? 4 : 1;
+  constexpr int V = Elem<T>::V, KG = 4 * V;
   constexpr int PC = lin_piece(NT), PITCH = PC + 4, LPR = PC / V, RPI = 64 / LPR;  // planes, lanes a row, rows an instruction of a piece
   constexpr bool FACTORS = MODE == 1 && X != FACTOR_NONE;
   using F = typename Frag<T>::type;
@@ -210,72 +211,107 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
   const bool stay = a.groups <= a.chunk_groups;
   const int tiles = (int)(stay ? (a.N + 31) / 32 : (a.N + LIN_ROWS - 1) / LIN_ROWS * 4);
 
+  // weights of k-groups g0 .. g0 + ng in the order of the A operands, several loads a thread in flight
   auto stage = [&](int g0, int ng) __attribute__((always_inline)) {
-#pragma unroll STAGE_UNROLL
-    for (int e = threadIdx.x; e < NT * ng * 64; e += 256) {
-      const int l = e & 63, t = (e >> 6) % NT, g = (e >> 6) / NT;
-      const int m = m0 + 16 * t + (l & 15), k = (g0 + g) * KG + (l >> 4) * V;
-      Pack<T, V> v;
-      if (MODE == 1) v = load_some<T, V>(wt + (int64_t)m * a.K + k, m < a.M ? a.K - k : 0);
-      else
+    constexpr int B = 4;
+    if (MODE == 1 || NT == 8 || a.transposed) {  // [M, K]: a lane's V elements lie together
+      for (int e0 = threadIdx.x; e0 < NT * ng * 64; e0 += 256 * B) {
+        Pack<T, V> v[B];
 #pragma unroll
-        for (int j = 0; j < V; ++j) v.v[j] = m < a.M && k + j < a.K ? wt[(int64_t)(k + j) * a.M + m] : (T)0.f;
-      __builtin_memcpy(&wl[e], &v, 16);
+        for (int i = 0; i < B; ++i) {
+          const int e = e0 + 256 * i, l = e & 63, t = (e >> 6) % NT, g = (e >> 6) / NT;
+          const int m = m0 + 16 * t + (l & 15), k = (g0 + g) * KG + (l >> 4) * V;
+          v[i] = load_some<T, V>(wt + (int64_t)m * a.K + k, e < NT * ng * 64 && m < a.M ? a.K - k : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+          if (e0 + 256 * i < NT * ng * 64) __builtin_memcpy(&wl[e0 + 256 * i], &v[i], 16);
+      }
+    } else {  // [K, M]: V planes of one k, spread over V lanes' places
+      constexpr int MV = NT * 16 / V;  // vectors a row
+      const int n = MV * ng * KG;
+      T *lds = (T *)wl;
+      for (int e = threadIdx.x; e < n; e += 256) {
+        const int m = e % MV * V, k = e / MV;
+        const Pack<T, V> v = load_some<T, V>(wt + (int64_t)(g0 * KG + k) * a.M + m0 + m, g0 * KG + k < a.K ? a.M - m0 - m : 0);
+#pragma unroll
+        for (int j = 0; j < V; ++j) lds[(((k / KG * NT + (m + j) / 16) * 64 + k % KG / V * 16 + (m + j) % 16) * V) + k % V] = v.v[j];
+      }
     }
   };
   if (stay) stage(0, a.groups);
   __syncthreads();
 
-  // a piece of results: 16 sites x PC planes from LDS, this lane's V planes of every RPI-th of them
-  auto finish = [&](auto drop, auto fac, int64_t row0, int pc) __attribute__((always_inline)) {
-    constexpr bool DROP = decltype(drop)::value, FAC = decltype(fac)::value;
-    const int r0 = lane / LPR, c = lane % LPR * V, m = m0 + pc + c, left = a.M - m;
+  // a piece of results: 16 sites x PC planes from LDS, this lane's V planes of every RPI-th of them.  WHOLE: all of them are there, and
+  // everything is requested before any of it is used
+  auto finish = [&](auto whole, auto drop, auto fac, int64_t row0, int pc) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(whole)::value, DROP = decltype(drop)::value, FAC = decltype(fac)::value;
+    constexpr int IT = 16 / RPI;
+    const int r0 = lane / LPR, c = lane % LPR * V, m = m0 + pc + c, left = WHOLE ? V : a.M - m;
+    const int rows = WHOLE ? 16 : (int)min((int64_t)16, a.N - row0);
     if (left <= 0) return;
-    const int rows = (int)min((int64_t)16, a.N - row0);
     // (scalar bases, 32-bit offsets)
     T *out = (T *)a.out + row0 * a.M + m0 + pc;
     Q *fo = (Q *)a.factor + row0 * a.M + m0 + pc;
     const T *res = (const T *)a.residual + row0 * a.ld_res + m0 + pc;
     const unsigned o0 = (unsigned)(r0 * a.M + c), res0 = (unsigned)(r0 * (int)a.ld_res + c);
+    Pack<T, V> rv[IT];
+    if (MODE == 0 && a.residual)
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const T *p = res + (int64_t)(i * RPI) * a.ld_res + res0;
+        rv[i] = WHOLE ? load_pack<T, V>(p) : load_some<T, V>(p, i * RPI + r0 < rows ? left : 0);
+      }
+    float z[IT][V];
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+      for (int j = 0; j < V; j += 4) {
+        const floatx4 v = *(const floatx4 *)(sw + (i * RPI + r0) * PITCH + c + j);
+        z[i][j] = v[0], z[i][j + 1] = v[1], z[i][j + 2] = v[2], z[i][j + 3] = v[3];
+      }
     PhiloxPlane plane[V / 4];
     if constexpr (DROP)
 #pragma unroll
       for (int q = 0; q < V / 4; ++q) plane[q] = philox_plane(key, (uint32_t)((m >> 2) + q));
 #pragma unroll
-    for (int it = 0; it < 16; it += RPI) {
-      if (it + r0 >= rows) break;
-      float z[V];
-#pragma unroll
-      for (int j = 0; j < V; j += 4) {
-        const floatx4 v = *(const floatx4 *)(sw + (it + r0) * PITCH + c + j);
-        z[j] = v[0], z[j + 1] = v[1], z[j + 2] = v[2], z[j + 3] = v[3];
-      }
+    for (int i = 0; i < IT; ++i) {
       Pack<T, V> y;
-      if constexpr (MODE == 1) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) y.v[j] = (T)z[j];
-      } else {
-        Pack<Q, V> f;
+      Pack<Q, V> f;
+      if constexpr (MODE == 0) {
         PhiloxSite site;
-        if constexpr (DROP) site = philox_site(key, (uint32_t)(row0 + it) + r0);
+        if constexpr (DROP) site = philox_site(key, (uint32_t)(row0 + i * RPI) + r0);
 #pragma unroll
         for (int q = 0; q < V / 4; ++q) {
           Words w;
           if constexpr (DROP) w = philox(key, plane[q], site);
 #pragma unroll
-          for (int j = 4 * q; j < 4 * q + 4; ++j) z[j] = activated<T, X, DROP>(z[j], !DROP || w.w[j & 3] >= a.threshold, a, f.v[j]);
+          for (int j = 4 * q; j < 4 * q + 4; ++j) z[i][j] = activated<T, X, DROP>(z[i][j], !DROP || w.w[j & 3] >= a.threshold, a, f.v[j]);
         }
-        if (a.residual) {
-          const Pack<T, V> rv = load_some<T, V>(res + it * a.ld_res + res0, left);
+        if (a.residual)
 #pragma unroll
-          for (int j = 0; j < V; ++j) z[j] += (float)rv.v[j];
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) y.v[j] = (T)z[j];
-        if constexpr (FAC) store_some<Q, V>(fo + (int64_t)it * a.M + o0, f, left);
+          for (int j = 0; j < V; ++j) z[i][j] += (float)rv[i].v[j];
       }
-      store_some<T, V>(out + (int64_t)it * a.M + o0, y, left);
+#pragma unroll
+      for (int j = 0; j < V; ++j) y.v[j] = (T)z[i][j];
+      T *o = out + (int64_t)(i * RPI) * a.M + o0;
+      Q *fp = fo + (int64_t)(i * RPI) * a.M + o0;
+      if constexpr (WHOLE) {
+        if constexpr (FAC) store_pack<Q, V>(fp, f);
+        store_pack<T, V>(o, y);
+      } else if (i * RPI + r0 < rows) {
+        if constexpr (FAC) store_some<Q, V>(fp, f, left);
+        store_some<T, V>(o, y, left);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // (one row's epilogue at a time)
     }
+  };
+  auto finish_as = [&](auto whole, int64_t row0, int pc) __attribute__((always_inline)) {
+    if constexpr (MODE == 1) finish(whole, std::false_type(), std::false_type(), row0, pc);
+    else if (a.threshold)
+      a.factor ? finish(whole, std::true_type(), std::true_type(), row0, pc) : finish(whole, std::true_type(), std::false_type(), row0, pc);
+    else
+      a.factor ? finish(whole, std::false_type(), std::true_type(), row0, pc) : finish(whole, std::false_type(), std::false_type(), row0, pc);
   };
 
   for (int tile = rb * 4 + wave; tile < tiles; tile += a.row_blocks * 4) {
@@ -349,9 +385,11 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
       }
       const F *wg = wl + lane;
       int g = 0;
-      if (NT < 8 && !(FACTORS && sizeof(T) == 2))
+      // (as many as the registers allow)
+      if (NT < 8 && !FACTORS)
         for (; g + 4 <= nf; g += 4, wg += 4 * NT * 64) batch(std::integral_constant<int, 4>(), std::true_type(), g0 + g, wg);
-      for (; g + 2 <= nf; g += 2, wg += 2 * NT * 64) batch(std::integral_constant<int, 2>(), std::true_type(), g0 + g, wg);
+      if (!(NT == 8 && FACTORS && sizeof(T) == 4))
+        for (; g + 2 <= nf; g += 2, wg += 2 * NT * 64) batch(std::integral_constant<int, 2>(), std::true_type(), g0 + g, wg);
       for (; g < nf; ++g, wg += NT * 64) batch(std::integral_constant<int, 1>(), std::true_type(), g0 + g, wg);
       if (g < ng) batch(std::integral_constant<int, 1>(), std::false_type(), g0 + g, wg);
     }
@@ -371,15 +409,26 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
       __builtin_amdgcn_wave_barrier();
       const int64_t r = row0 + piece / PPU * 16;
       const int pc = piece % PPU * PC;
-      if (MODE == 1) finish(std::false_type(), std::false_type(), r, pc);
-      else if (a.threshold)
-        a.factor ? finish(std::true_type(), std::true_type(), r, pc) : finish(std::true_type(), std::false_type(), r, pc);
-      else
-        a.factor ? finish(std::false_type(), std::true_type(), r, pc) : finish(std::false_type(), std::false_type(), r, pc);
+      if (r + 16 <= a.N && m0 + pc + PC <= a.M) finish_as(std::true_type(), r, pc);
+      else finish_as(std::false_type(), r, pc);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
   }
+}
+
+// weight [K, M] -> [M, K], 32 x 32 at a time
+template <class T>
+__global__ void __launch_bounds__(256) k_linear_transpose(const T *w, T *out, int K, int M) {
+  __shared__ T tile[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5, k0 = blockIdx.y * 32, m0 = blockIdx.x * 32;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    if (k0 + y + i < K && m0 + x < M) tile[y + i][x] = w[(int64_t)(k0 + y + i) * M + m0 + x];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    if (m0 + y + i < M && k0 + x < K) out[(int64_t)(m0 + y + i) * K + k0 + x] = tile[x][y + i];
 }
 
 // Up to R rows (a serving loop's single sites): bound by one trip to memory for the weights, which the tiles above would make with a
@@ -674,7 +723,8 @@ static int linear_by_width(const LinearArgs &a, hipStream_t st) {
   const int64_t tiles = (a.N + LIN_ROWS - 1) / LIN_ROWS;
   auto blocks = [&](int nt) { return (a.M + 16 * nt - 1) / (16 * nt); };
   if (a.M <= 32 || tiles * blocks(4) < 256) return linear_launch<T, 2, MODE, X>(a, st);
-  if (a.M <= 64 || tiles * blocks(8) < 256 || blocks(4) < 2 * blocks(8)) return linear_launch<T, 4, MODE, X>(a, st);
+  if (a.M <= 64 || tiles * blocks(8) < 256 || blocks(4) < 2 * blocks(8) || (MODE == 0 && !a.transposed))
+    return linear_launch<T, 4, MODE, X>(a, st);
   return linear_launch<T, 8, MODE, X>(a, st);
 }
 template <class T, int ACT>
@@ -686,6 +736,10 @@ static int linear_forward(const LinearArgs &a, hipStream_t st) {
   SCN_CHECK_LAUNCH();
   return 0;
 }
+
+// From this many sites on a launch that lays the weights out as [n_out, n_in] pays for itself (2 us; every workgroup then fetches them
+// by 16 bytes of a reduction instead of by single values)
+constexpr int64_t LIN_TRANSPOSE_ROWS = 4096;
 
 static FactorScale factor_scale(double leak, double p) {
   const double up = 1.0 / (1.0 - p);
@@ -751,9 +805,13 @@ int scn_rng_take(int64_t *state, int64_t *used, void *stream) {
   return 0;
 }
 
+size_t scn_linear_forward_temp_bytes(int64_t N, int n_in, int n_out, int dtype) {
+  return N < LIN_TRANSPOSE_ROWS ? 0 : (size_t)n_in * n_out * (dtype == SCN_F32 ? 4 : 2);
+}
+
 int scn_linear_forward(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_res,
                        void *y, void *factor, int64_t N, int n_in, int n_out, int act, double leakiness, double p,
-                       const int64_t *rng, int dtype, void *stream) {
+                       const int64_t *rng, int dtype, void *temp, size_t temp_bytes, void *stream) {
   if (int e = lin_check(N, n_in, n_out, dtype)) return e;
   SCN_REQUIRE(act == SCN_ACT_LEAKY || act == SCN_ACT_SILU || act == SCN_ACT_GELU, "linear: activation");
   SCN_REQUIRE(p >= 0 && p < 1 && (p == 0 || rng), "linear: 0 <= p < 1, with random words if it is not 0");
@@ -775,8 +833,17 @@ int scn_linear_forward(const void *x, int64_t ldx, const void *weight, const voi
   a.threshold = drop_threshold(p);
   a.leak = (float)leakiness;
   a.up = (float)(1.0 / (1.0 - p));
+  const bool transpose = N >= LIN_TRANSPOSE_ROWS;
+  SCN_REQUIRE(!transpose || (temp && temp_bytes >= scn_linear_forward_temp_bytes(N, n_in, n_out, dtype)), "linear: workspace");
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
+    if (transpose) {
+      k_linear_transpose<T><<<dim3((n_out + 31) / 32, (n_in + 31) / 32), 256, 0, as_stream(stream)>>>((const T *)weight, (T *)temp, n_in,
+                                                                                                    n_out);
+      SCN_CHECK_LAUNCH();
+      a.weight = temp;
+      a.transposed = 1;
+    }
     if (act == SCN_ACT_SILU) return linear_forward<T, SCN_ACT_SILU>(a, as_stream(stream));
     if (act == SCN_ACT_GELU) return linear_forward<T, SCN_ACT_GELU>(a, as_stream(stream));
     if (a.leak == 1.f) return linear_forward<T, ACT_NONE>(a, as_stream(stream));

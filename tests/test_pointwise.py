@@ -82,8 +82,8 @@ def test_boundary_refuses_on_the_host():
     assert lib.scn_dropout(None, 8, None, 10, 8, 0, 0.5, None, None) == 2
     assert lib.scn_dropout(None, 8, None, 10, 8, 0, 1.0, None, None) == 2
     assert lib.scn_dropout(None, 8, None, 0, 8, 0, 0.5, None, None) == 0
-    assert lib.scn_linear_forward(None, 8, None, None, None, 0, None, None, 10, 8, 4, 0, 1.0, 0.0, None, 0, None) == 2
-    assert lib.scn_linear_forward(None, 8, None, None, None, 0, None, None, 10, 0, 4, 0, 1.0, 0.0, None, 0, None) == 2
+    assert lib.scn_linear_forward(None, 8, None, None, None, 0, None, None, 10, 8, 4, 0, 1.0, 0.0, None, 0, None, 0, None) == 2
+    assert lib.scn_linear_forward(None, 8, None, None, None, 0, None, None, 10, 0, 4, 0, 1.0, 0.0, None, 0, None, 0, None) == 2
     assert lib.scn_linear_dinput(None, 4, None, None, None, 10, 8, 4, 0, 1.0, 0.0, 5, None) == 2
     assert lib.scn_linear_dweight(None, 8, None, 4, None, None, None, 10, 8, 4, 0, 1.0, 0.0, 0, None, 0, None) == 2
     assert lib.scn_rng_take(None, None, None) == 2
