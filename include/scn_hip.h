@@ -490,7 +490,7 @@ int scn_rng_take(int64_t *state, int64_t *used, void *stream);
 
 /* y = residual + drop(act(x weight + bias)): weight [n_in, n_out], bias [n_out] or NULL, residual rows at ld_res elements or NULL,
  * drop as scn_dropout (p 0: none, rng NULL).  factor (NULL: not wanted) [N, n_out], of the size of `dtype`'s values, receives
- * d y / d (x weight + bias) in a form of its own for the two calls below, which need the same act, leakiness and p.  All else of
+ * act'(x weight + bias), 0 where dropped, in a form of its own for the two calls below, which need the same act, leakiness and p.  All else of
  * `dtype`; x rows at ldx elements, y and factor contiguous.  temp: scn_linear_forward_temp_bytes (0: may be NULL). */
 size_t scn_linear_forward_temp_bytes(int64_t N, int n_in, int n_out, int dtype);
 int scn_linear_forward(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_res,

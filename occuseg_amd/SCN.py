@@ -2045,8 +2045,8 @@ def _linear_args(what, features, weight, bias):
 def FusedNetworkInNetwork_updateOutput(input_features, output_features, weight, bias, residual, activation, leakiness, p, rng,
                                        factor=None):
     """output = residual + dropout(act(input @ weight + bias)) in one kernel.  ``residual`` None: none; ``p`` 0: no dropout, ``rng``
-    None.  ``factor`` (an empty tensor of factor_dtype(input), training) receives d output / d (input @ weight + bias) for the backward
-    pass: float32, or 16-bit codes beside 16-bit features."""
+    None.  ``factor`` (an empty tensor of factor_dtype(input), training) receives what the backward pass needs of activation and mask
+    (float32, or 16-bit codes beside 16-bit features)."""
     what = "FusedNetworkInNetwork_updateOutput"
     code, N, Ci, Co = _linear_args(what, input_features, weight, bias)
     act, p = _activation(what, activation), _drop_p(what, p)

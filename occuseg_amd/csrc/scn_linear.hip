@@ -1,6 +1,7 @@
 // 1x1 convolution with its epilogue, y = residual + drop(act(x W + b)), its gradients, and dropout alone (gfx950).
 //
-//   backward:  f = drop'(.) act'(x W + b), left by the forward pass;  dz = dy f;  dx = dz W^T;  dW = x^T dz;  db = column sums of dz
+//   backward:  f = act'(x W + b), 0 where dropped, left by the forward pass;  dz = dy f / (1 - p);
+//              dx = dz W^T;  dW = x^T dz;  db = column sums of dz
 //
 // Sites are many (up to 600k) and planes few (16 to 512), so the products are HBM bound but for the widest: 2 n_in n_out flops for
 // n_in + n_out values, 16 to 128 flops a byte where fp32 MFMA balances at 20 and bf16 at 300.  Everything that belongs to a row is
@@ -110,22 +111,23 @@ __device__ __forceinline__ void store_some(T *p, const Pack<T, V> &v, int n) {
       if (j < n) p[j] = v.v[j];
 }
 
-// What the backward pass needs of activation and mask, one value per output: f = dy / d(x W + b).  fp32: f itself.  16-bit features:
-// rounding f to them, then dy f to them, would make the second of these roundings twice; 16 bits of fixed point are finer.
-//   FACTOR_FIXED  f = up q 2^-14, up = 1 / (1 - p); |slope| <= 1.13 for the smooth activations; q = -2^15: NaN
-//   FACTOR_SIGN   q = 2: f = up, 1: up leak, 0: dropped     (leaky ReLU, whose slope may be any number)
-enum { FACTOR_NONE, FACTOR_FLOAT, FACTOR_FIXED, FACTOR_SIGN };
+// What the backward pass needs of activation and mask, one value per output: the slope, 0 for a dropped element.  (dy slope is what is
+// multiplied with; 1 / (1 - p) is applied to the sums.)  dz = dy slope is rounded to the features' type as the matrix units' operand;
+// slopes rounded to the same type would make that rounding twice, so they are kept finer:
+//   FACTOR_FLOAT  fp32 features: fp32
+//   FACTOR_HALF   bf16 features: fp16, 2^-12 of a slope
+//   FACTOR_FIXED  fp16 features: 16 bits of fixed point, 2^-15 (the smooth activations' slopes are below 1.13); -2^15: NaN
+//   FACTOR_SIGN   leaky ReLU of 16-bit features, whose slope may be any number: 2: 1, 1: leak, 0: dropped
+enum { FACTOR_NONE, FACTOR_FLOAT, FACTOR_HALF, FACTOR_FIXED, FACTOR_SIGN };
 template <class T> struct FactorOf { using type = int16_t; };
 template <> struct FactorOf<float> { using type = float; };
 
-struct FactorScale {
-  float unit, up, low;
-};
 template <int FACTOR, class Q>
-__device__ __forceinline__ float factor_value(Q q, const FactorScale &s) {
+__device__ __forceinline__ float factor_value(Q q, float leak) {
   if constexpr (FACTOR == FACTOR_FLOAT) return (float)q;
-  if constexpr (FACTOR == FACTOR_SIGN) return q == 2 ? s.up : q == 1 ? s.low : 0.f;
-  return (int)q == -32768 ? __builtin_nanf("") : (float)(int)q * s.unit;
+  if constexpr (FACTOR == FACTOR_HALF) return (float)__builtin_bit_cast(_Float16, q);
+  if constexpr (FACTOR == FACTOR_SIGN) return q == 2 ? 1.f : q == 1 ? leak : 0.f;
+  return (int)q == -32768 ? __builtin_nanf("") : (float)(int)q * (1.f / 16384.f);
 }
 
 struct LinearArgs {
@@ -143,7 +145,6 @@ struct LinearArgs {
   int col_blocks, row_blocks;
   uint32_t threshold;
   float leak, up;
-  FactorScale scale;
 };
 
 constexpr int ACT_NONE = 3;  // SCN_ACT_LEAKY with slope 1
@@ -154,14 +155,12 @@ __device__ __forceinline__ float activated(float z, bool keep, const LinearArgs 
   float value = z, slope = 1.f;
   if constexpr (ACT != ACT_NONE) act_value_slope<ACT, sizeof(T) == 4>(z, a.leak, value, slope);
   if constexpr (DROP) value = keep ? value * a.up : 0.f;
-  if constexpr (sizeof(T) == 4) {
-    factor = DROP ? (keep ? slope * a.up : 0.f) : slope;
-  } else {
-    if constexpr (ACT == ACT_NONE) factor = 2;
-    else if constexpr (ACT == SCN_ACT_LEAKY) factor = z > 0 ? 2 : 1;
-    else factor = slope == slope ? (int16_t)(int)rintf(slope * 16384.f) : -32768;
-    if (DROP && !keep) factor = 0;
-  }
+  if constexpr (sizeof(T) == 4) factor = slope;
+  else if constexpr (ACT == ACT_NONE) factor = 2;
+  else if constexpr (ACT == SCN_ACT_LEAKY) factor = z > 0 ? 2 : 1;
+  else if constexpr (std::is_same<T, __bf16>::value) factor = __builtin_bit_cast(int16_t, (_Float16)slope);
+  else factor = slope == slope ? (int16_t)(int)rintf(slope * 16384.f) : -32768;
+  if (DROP && !keep) factor = 0;
   return value;
 }
 
@@ -293,7 +292,7 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
           for (int j = 0; j < V; ++j) z[i][j] += (float)rv[i].v[j];
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) y.v[j] = (T)z[i][j];
+      for (int j = 0; j < V; ++j) y.v[j] = (T)(MODE == 1 ? z[i][j] * a.up : z[i][j]);
       T *o = out + (int64_t)(i * RPI) * a.M + o0;
       Q *fp = fo + (int64_t)(i * RPI) * a.M + o0;
       if constexpr (WHOLE) {
@@ -355,7 +354,7 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
         for (int u = 0; u < 2; ++u) {
           if constexpr (FACTORS)
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[i][u].v[j] = (T)((float)v[i][u].v[j] * factor_value<X>(f[i][u].v[j], a.scale));
+            for (int j = 0; j < V; ++j) v[i][u].v[j] = (T)((float)v[i][u].v[j] * factor_value<X>(f[i][u].v[j], a.leak));
           __builtin_memcpy(&b[u], &v[i][u], 16);
         }
 #pragma unroll
@@ -501,7 +500,7 @@ struct DwArgs {
   int64_t slice_rows;
   float *slab;      // [slices][Ci][Co], then [slices][Co]
   int want_bias;
-  FactorScale scale;
+  float leak, up;
 };
 
 // rows r for which the 64 planes from c0 of rows up to r lie in the memory of a [N, C] tensor with rows at ld
@@ -571,7 +570,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_dw(DwArgs a) {
 #pragma unroll
       for (int e = 0; e < RE; ++e)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) vd[e].v[j] = (T)((float)vd[e].v[j] * factor_value<FACTOR>(vf[e].v[j], a.scale));
+        for (int j = 0; j < 4; ++j) vd[e].v[j] = (T)((float)vd[e].v[j] * factor_value<FACTOR>(vf[e].v[j], a.leak));
     if constexpr (F32) {
 #pragma unroll
       for (int e = 0; e < RE; ++e) {
@@ -649,12 +648,12 @@ __global__ void __launch_bounds__(256, 2) k_linear_dw(DwArgs a) {
     for (int q = 0; q < 4; ++q) {
       const int row = ci0 + 64 * (i / 4) + 16 * lq + 4 * q + (i & 3);  // A row 4 lq + q of tile i
       if (row < a.Ci && no > 0) {
-        Pack<float, 4> v = {{acc[i][0][q], acc[i][1][q], acc[i][2][q], acc[i][3][q]}};
+        Pack<float, 4> v = {{acc[i][0][q] * a.up, acc[i][1][q] * a.up, acc[i][2][q] * a.up, acc[i][3][q] * a.up}};
         store_some<float, 4>(slab + (int64_t)row * a.Co + co, v, no);
       }
     }
   if (bias && lq == 0 && no > 0) {
-    Pack<float, 4> v = {{sums[0], sums[1], sums[2], sums[3]}};
+    Pack<float, 4> v = {{sums[0] * a.up, sums[1] * a.up, sums[2] * a.up, sums[3] * a.up}};
     store_some<float, 4>(a.slab + (int64_t)a.slices * a.Ci * a.Co + (int64_t)slice * a.Co + co, v, no);
   }
 }
@@ -741,16 +740,15 @@ static int linear_forward(const LinearArgs &a, hipStream_t st) {
 // by 16 bytes of a reduction instead of by single values)
 constexpr int64_t LIN_TRANSPOSE_ROWS = 4096;
 
-static FactorScale factor_scale(double leak, double p) {
-  const double up = 1.0 / (1.0 - p);
-  return FactorScale{(float)(up / 16384.0), (float)up, (float)(up * leak)};
-}
+// 1 / (1 - p); without factors the pass had no dropout
+static float keep_scale(const void *factor, double p) { return factor ? (float)(1.0 / (1.0 - p)) : 1.f; }
 // f(how the factors are stored)
 template <class T, class F>
 static int by_factor(const void *factor, int act, F &&f) {
   if (!factor) return f(std::integral_constant<int, FACTOR_NONE>());
   if constexpr (sizeof(T) == 4) return f(std::integral_constant<int, FACTOR_FLOAT>());
-  else return act == SCN_ACT_LEAKY ? f(std::integral_constant<int, FACTOR_SIGN>()) : f(std::integral_constant<int, FACTOR_FIXED>());
+  else if (act == SCN_ACT_LEAKY) return f(std::integral_constant<int, FACTOR_SIGN>());
+  else return f(std::integral_constant<int, std::is_same<T, __bf16>::value ? FACTOR_HALF : FACTOR_FIXED>());
 }
 
 // planes a tile of dW takes of x: 128 read d_y and the factors half as often; with 16-bit features and factors that is more than the
@@ -861,7 +859,8 @@ int scn_linear_dinput(const void *d_y, int64_t ld_dy, const void *factor, const 
   a.in = d_y;
   a.ld_in = ld_dy;
   a.factor_in = factor;
-  a.scale = factor_scale(leakiness, p);
+  a.leak = (float)leakiness;
+  a.up = keep_scale(factor, p);
   a.weight = weight;
   a.out = d_x;
   a.N = N;
@@ -888,7 +887,8 @@ int scn_linear_dweight(const void *x, int64_t ldx, const void *d_y, int64_t ld_d
   a.x = x;
   a.dy = d_y;
   a.factor = factor;
-  a.scale = factor_scale(leakiness, p);
+  a.leak = (float)leakiness;
+  a.up = keep_scale(factor, p);
   a.ldx = ldx;
   a.ld_dy = ld_dy;
   a.N = N;

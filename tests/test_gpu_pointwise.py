@@ -294,8 +294,9 @@ def check_linear(got, x, w, b, res, activation, leakiness, keep, p, dy, what):
     smooth = activation != "leaky_relu"
     ev = up * (1.13 * ez + (8 * U + approx) * (o["z"].abs() + 1) * smooth) + 4 * U * o["value"].abs()
     check(got[0], o["y"], 1.01 * (ev + 2 * U * (o["value"].abs() + o["y"].abs()) + h * o["y"].abs()) + 1e-30, what + " y")
-    # dz: the stored factor and the operand are rounded to the type (fp32: two roundings of U); nothing is, without a factor
-    ef = up * (0.8 * ez + (8 * U + approx) * (1 + o["z"].abs())) * smooth
+    # dz: the stored slope (bf16: in fp16, within h; fp16: in steps of 2^-14) and the operand are rounded (fp32: two roundings of U);
+    # nothing is, without a factor
+    ef = up * (0.8 * ez + (8 * U + approx) * (1 + o["z"].abs()) + (2.0 ** -15 if t == torch.float16 else 0)) * smooth
     tiny = torch.finfo(t).smallest_normal * h  # below the normal numbers a rounding is half the smallest subnormal
     bare = activation == "leaky_relu" and leakiness == 1 and keep is None
     edz = torch.zeros_like(dy) if bare else dy.abs() * (ef + h * o["f"].abs() + 2 * tiny) + (h + 2 * U) * o["dz"].abs() + 2 * tiny
