@@ -1892,13 +1892,13 @@ def _pointwise(what, x, *others):
         raise RuntimeError("occuseg_amd.SCN.%s: features must be a [sites, planes] tensor" % what)
     if not x.is_cuda:
         raise RuntimeError("occuseg_amd.SCN.%s: features must live on the GPU -- this backend has no CPU path" % what)
-    code = _DTYPES.get(x.dtype)
+    dtype, device = x.dtype, x.get_device()
+    code = _DTYPES.get(dtype)
     if code is None:
-        raise RuntimeError("occuseg_amd.SCN.%s: float32, bfloat16 or float16 features, not %s" % (what, x.dtype))
+        raise RuntimeError("occuseg_amd.SCN.%s: float32, bfloat16 or float16 features, not %s" % (what, dtype))
     for t in others:
-        if t is not None and t.numel() and (t.device != x.device or t.dtype != x.dtype):
-            raise RuntimeError("occuseg_amd.SCN.%s: a %s tensor on %s beside %s features on %s" % (what, t.dtype, t.device, x.dtype,
-                                                                                              x.device))
+        if t is not None and (t.dtype is not dtype or t.get_device() != device) and t.numel():
+            raise RuntimeError("occuseg_amd.SCN.%s: a %s tensor on %s beside %s features on %s" % (what, t.dtype, t.device, dtype, x.device))
     return code
 
 
@@ -1924,15 +1924,25 @@ _NO_DEVICE_CHANGE = contextlib.nullcontext()
 
 def _on(t):
     """launches go to the current stream of the tensor's device, whichever device is current"""
-    return _NO_DEVICE_CHANGE if t.device.index == _lib._cur_device() else torch.cuda.device(t.device)
+    return _NO_DEVICE_CHANGE if t.get_device() == _lib._cur_device() else torch.cuda.device(t.device)
 
 
 def _opt(t):
     return t if t is not None and t.numel() else None
 
 
+def _sized(t, *shape):
+    """callers pass empty outputs which are resized here, or outputs of the right shape"""
+    if t.shape != shape:
+        t.resize_(*shape)
+    elif not t.is_contiguous():
+        raise RuntimeError("occuseg_amd.SCN: outputs must be contiguous")
+    return t
+
+
 def _rng(what, rng, x):
-    if not (torch.is_tensor(rng) and rng.dtype == torch.int64 and rng.numel() == 2 and rng.is_contiguous() and rng.device == x.device):
+    if not (torch.is_tensor(rng) and rng.dtype is torch.int64 and rng.numel() == 2 and rng.is_contiguous()
+            and rng.get_device() == x.get_device()):
         raise RuntimeError("occuseg_amd.SCN.%s: rng must be an int64 tensor (seed, offset) on the features' device" % what)
     return rng
 
@@ -1947,56 +1957,60 @@ def _drop_p(what, p):
 def _group_norm_args(what, features, offsets, weight, bias, groups, activation):
     code = _pointwise(what, features)
     N, C = features.shape
+    device = features.get_device()
     groups = int(groups)
     if groups < 1 or C < 1 or C % groups:
         raise RuntimeError("occuseg_amd.SCN.%s: %d planes do not divide into %d groups" % (what, C, groups))
-    if not (torch.is_tensor(offsets) and offsets.dtype == torch.int64 and offsets.dim() == 1 and offsets.numel() >= 2
-            and offsets.is_contiguous() and offsets.device == features.device):
+    if not (torch.is_tensor(offsets) and offsets.dtype is torch.int64 and offsets.dim() == 1 and offsets.numel() >= 2
+            and offsets.is_contiguous() and offsets.get_device() == device):
         raise RuntimeError("occuseg_amd.SCN.%s: offsets must be an int64 tensor [samples + 1] on the features' device" % what)
-    for t in (_opt(weight), _opt(bias)):
-        if t is not None and not (t.dtype == torch.float32 and t.numel() == C and t.is_contiguous() and t.device == features.device):
+    weight, bias = _opt(weight), _opt(bias)
+    for t in (weight, bias):
+        if t is not None and not (t.dtype is torch.float32 and t.numel() == C and t.is_contiguous() and t.get_device() == device):
             raise RuntimeError("occuseg_amd.SCN.%s: weight and bias must be float32 [%d] on the features' device" % (what, C))
-    return code, N, C, groups, offsets.numel() - 1, _activation(what, activation)
+    return code, N, C, groups, offsets.numel() - 1, _activation(what, activation), weight, bias
 
 
 def GroupNormalization_updateOutput(input_features, output_features, stats, offsets, weight, bias, eps, groups, activation, leakiness):
     """Normalise each of ``groups`` groups of consecutive planes over the sites of each sample, scale, shift, activate.  ``offsets``
-    int64 [samples + 1]: see Metadata_3.sampleOffsets; rows outside of 0..offsets[-1] are left as ``resize_`` leaves them.
+    int64 [samples + 1]: see Metadata_3.sampleOffsets; rows outside of offsets[0]..offsets[-1] are not written.
     ``stats`` receives (mean, 1 / sqrt(var + eps)) as float32 [samples, groups, 2], which the backward pass takes."""
     what = "GroupNormalization_updateOutput"
-    code, N, C, groups, S, act = _group_norm_args(what, input_features, offsets, weight, bias, groups, activation)
+    code, N, C, groups, S, act, weight, bias = _group_norm_args(what, input_features, offsets, weight, bias, groups, activation)
     x = input_features.contiguous()
     lib = _lib_()
     with _on(x):
-        output_features.resize_(N, C)
-        stats.resize_(S, groups, 2)
+        _sized(output_features, N, C)
+        _sized(stats, S, groups, 2)
         tb = lib.scn_group_norm_temp_bytes(N, C, groups, S, code, 0)
         temp = torch.empty(tb, dtype=torch.uint8, device=x.device)
         ev = _prof_begin("bn")
-        check(lib.scn_group_norm_forward(ptr(x), ptr(output_features), ptr(stats), ptr(offsets), ptr(_opt(weight)), ptr(_opt(bias)),
+        check(lib.scn_group_norm_forward(ptr(x), ptr(output_features), ptr(stats), ptr(offsets), ptr(weight), ptr(bias),
                                          float(eps), act, float(leakiness), N, C, groups, S, code, ptr(temp), tb, stream()))
-        _prof_end(ev, "gn_fwd", 0.0, 3.0 * N * C * x.element_size(), (N, C, groups))
+        if ev is not None:
+            _prof_end(ev, "gn_fwd", 0.0, 3.0 * N * C * x.element_size(), (N, C, groups))
 
 
 def GroupNormalization_backward(input_features, d_input_features, d_output_features, stats, offsets, weight, bias, d_weight, d_bias,
                                 groups, activation, leakiness):
     """d_weight / d_bias (float32 [planes], empty: not wanted) are assigned"""
     what = "GroupNormalization_backward"
-    code, N, C, groups, S, act = _group_norm_args(what, input_features, offsets, weight, bias, groups, activation)
+    code, N, C, groups, S, act, weight, bias = _group_norm_args(what, input_features, offsets, weight, bias, groups, activation)
     _pointwise(what, d_output_features, input_features)
     if d_output_features.shape != input_features.shape or stats.numel() != 2 * S * groups or stats.dtype != torch.float32:
         raise RuntimeError("occuseg_amd.SCN.%s: shapes" % what)
     x, dy = input_features.contiguous(), d_output_features.contiguous()
     lib = _lib_()
     with _on(x):
-        d_input_features.resize_(N, C)
+        _sized(d_input_features, N, C)
         tb = lib.scn_group_norm_temp_bytes(N, C, groups, S, code, 1)
         temp = torch.empty(tb, dtype=torch.uint8, device=x.device)
         ev = _prof_begin("bn")
-        check(lib.scn_group_norm_backward(ptr(x), ptr(dy), ptr(d_input_features), ptr(stats), ptr(offsets), ptr(_opt(weight)),
-                                          ptr(_opt(bias)), ptr(_opt(d_weight)), ptr(_opt(d_bias)), act, float(leakiness), N, C, groups,
+        check(lib.scn_group_norm_backward(ptr(x), ptr(dy), ptr(d_input_features), ptr(stats), ptr(offsets), ptr(weight),
+                                          ptr(bias), ptr(_opt(d_weight)), ptr(_opt(d_bias)), act, float(leakiness), N, C, groups,
                                           S, code, ptr(temp), tb, stream()))
-        _prof_end(ev, "gn_bwd", 0.0, 5.0 * N * C * x.element_size(), (N, C, groups))
+        if ev is not None:
+            _prof_end(ev, "gn_bwd", 0.0, 5.0 * N * C * x.element_size(), (N, C, groups))
 
 
 def Dropout_updateOutput(input_features, output_features, p, rng):
@@ -2008,7 +2022,7 @@ def Dropout_updateOutput(input_features, output_features, p, rng):
     x, ld = _rows(input_features)
     N, C = x.shape
     with _on(x):
-        output_features.resize_(N, C)
+        _sized(output_features, N, C)
         if C:
             check(_lib_().scn_dropout(ptr(x), ld, ptr(output_features), N, C, code, p, ptr(rng), stream()))
 
@@ -2035,11 +2049,12 @@ def factor_dtype(features):
 
 def _linear_args(what, features, weight, bias):
     code = _pointwise(what, features, weight, bias)
-    if weight.dim() != 2 or weight.size(0) < 1 or weight.size(1) < 1 or features.size(1) != weight.size(0):
-        raise RuntimeError("occuseg_amd.SCN.%s: features %s and weight %s" % (what, tuple(features.shape), tuple(weight.shape)))
-    if _opt(bias) is not None and bias.numel() != weight.size(1):
-        raise RuntimeError("occuseg_amd.SCN.%s: weight %s and bias %s" % (what, tuple(weight.shape), tuple(bias.shape)))
-    return code, features.size(0), weight.size(0), weight.size(1)
+    shape = tuple(weight.shape)
+    if len(shape) != 2 or shape[0] < 1 or shape[1] < 1 or features.size(1) != shape[0]:
+        raise RuntimeError("occuseg_amd.SCN.%s: features %s and weight %s" % (what, tuple(features.shape), shape))
+    if bias is not None and bias.numel() != shape[1]:
+        raise RuntimeError("occuseg_amd.SCN.%s: weight %s and bias %s" % (what, shape, tuple(bias.shape)))
+    return code, features.size(0), shape[0], shape[1]
 
 
 def FusedNetworkInNetwork_updateOutput(input_features, output_features, weight, bias, residual, activation, leakiness, p, rng,
@@ -2048,31 +2063,35 @@ def FusedNetworkInNetwork_updateOutput(input_features, output_features, weight, 
     None.  ``factor`` (an empty tensor of factor_dtype(input), training) receives what the backward pass needs of activation and mask
     (float32, or 16-bit codes beside 16-bit features)."""
     what = "FusedNetworkInNetwork_updateOutput"
+    bias = _opt(bias)
     code, N, Ci, Co = _linear_args(what, input_features, weight, bias)
     act, p = _activation(what, activation), _drop_p(what, p)
     rng = _rng(what, rng, input_features) if p > 0 else None
     x, ld = _rows(input_features)
-    bias = bias.contiguous() if _opt(bias) is not None else None
     res, ld_res = None, 0
+    if bias is not None:
+        bias = bias.contiguous()
     if residual is not None:
         _pointwise(what, residual, x)
-        if tuple(residual.shape) != (N, Co):
+        if residual.shape != (N, Co):
             raise RuntimeError("occuseg_amd.SCN.%s: residual %s for an output of %s" % (what, tuple(residual.shape), (N, Co)))
         res, ld_res = _rows(residual)
+    if factor is not None and (factor.dtype is not factor_dtype(x) or factor.get_device() != x.get_device()):
+        raise RuntimeError("occuseg_amd.SCN.%s: factor must be %s" % (what, factor_dtype(x)))
+    weight = weight.contiguous()
+    lib = _lib_()
     with _on(x):
-        output_features.resize_(N, Co)
+        _sized(output_features, N, Co)
         if factor is not None:
-            if factor.dtype != factor_dtype(x) or factor.device != x.device:
-                raise RuntimeError("occuseg_amd.SCN.%s: factor must be %s" % (what, factor_dtype(x)))
-            factor.resize_(N, Co)
-        lib = _lib_()
+            _sized(factor, N, Co)
         tb = lib.scn_linear_forward_temp_bytes(N, Ci, Co, code)
         temp = torch.empty(tb, dtype=torch.uint8, device=x.device) if tb else None
         ev = _prof_begin()
-        check(lib.scn_linear_forward(ptr(x), ld, ptr(weight.contiguous()), ptr(bias), ptr(res), ld_res, ptr(output_features),
-                                         ptr(factor), N, Ci, Co, act, float(leakiness), p, ptr(rng), code, ptr(temp), tb, stream()))
-        _prof_end(ev, "linear_fwd", 2.0 * N * Ci * Co,
-                  float(x.element_size()) * (N * (Ci + Co * (1 + (res is not None) + (factor is not None))) + Ci * Co), (N, Ci, Co))
+        check(lib.scn_linear_forward(ptr(x), ld, ptr(weight), ptr(bias), ptr(res), ld_res, ptr(output_features), ptr(factor), N, Ci, Co,
+                                     act, float(leakiness), p, ptr(rng), code, ptr(temp), tb, stream()))
+        if ev is not None:
+            _prof_end(ev, "linear_fwd", 2.0 * N * Ci * Co,
+                      float(x.element_size()) * (N * (Ci + Co * (1 + (res is not None) + (factor is not None))) + Ci * Co), (N, Ci, Co))
     return float(N) * Ci * Co
 
 
@@ -2084,31 +2103,32 @@ def FusedNetworkInNetwork_backward(input_features, d_input_features, d_output_fe
     code, N, Ci, Co = _linear_args(what, input_features, weight, None)
     act, p, leakiness = _activation(what, activation), _drop_p(what, p), float(leakiness)
     _pointwise(what, d_output_features, input_features)
-    if tuple(d_output_features.shape) != (N, Co) or (factor is not None and not (
-            tuple(factor.shape) == (N, Co) and factor.dtype == factor_dtype(input_features) and factor.is_contiguous()
-            and factor.device == input_features.device)):
+    if d_output_features.shape != (N, Co) or (factor is not None and not (
+            factor.shape == (N, Co) and factor.dtype is factor_dtype(input_features) and factor.is_contiguous()
+            and factor.get_device() == input_features.get_device())):
         raise RuntimeError("occuseg_amd.SCN.%s: shapes" % what)
     x, ldx = _rows(input_features)
     dy, ld_dy = _rows(d_output_features)
     lib = _lib_()
     with _on(x):
-        es = float(x.element_size())
+        nbytes = float(x.element_size()) * (N * (Ci + Co * (1 + (factor is not None))) + Ci * Co) if PROFILE is not None else 0.0
         if d_input_features is not None:
-            d_input_features.resize_(N, Ci)
+            weight = weight.contiguous()
+            _sized(d_input_features, N, Ci)
             ev = _prof_begin()
-            check(lib.scn_linear_dinput(ptr(dy), ld_dy, ptr(factor), ptr(weight.contiguous()), ptr(d_input_features), N, Ci, Co, act,
+            check(lib.scn_linear_dinput(ptr(dy), ld_dy, ptr(factor), ptr(weight), ptr(d_input_features), N, Ci, Co, act,
                                         leakiness, p, code, stream()))
-            _prof_end(ev, "linear_dx", 2.0 * N * Ci * Co, es * (N * (Ci + Co * (1 + (factor is not None))) + Ci * Co), (N, Ci, Co))
+            _prof_end(ev, "linear_dx", 2.0 * N * Ci * Co, nbytes, (N, Ci, Co))
         if d_weight is not None:
-            d_weight.resize_(Ci, Co)
+            _sized(d_weight, Ci, Co)
             if d_bias is not None:
-                d_bias.resize_(Co)
+                _sized(d_bias, Co)
             tb = lib.scn_linear_dweight_temp_bytes(N, Ci, Co)
             temp = torch.empty(tb, dtype=torch.uint8, device=x.device)
             ev = _prof_begin()
             check(lib.scn_linear_dweight(ptr(x), ldx, ptr(dy), ld_dy, ptr(factor), ptr(d_weight), ptr(d_bias), N, Ci, Co, act,
                                          leakiness, p, code, ptr(temp), tb, stream()))
-            _prof_end(ev, "linear_dw", 2.0 * N * Ci * Co, es * (N * (Ci + Co * (1 + (factor is not None))) + Ci * Co), (N, Ci, Co))
+            _prof_end(ev, "linear_dw", 2.0 * N * Ci * Co, nbytes, (N, Ci, Co))
 
 
 def _not_in_scope(name):

@@ -547,56 +547,62 @@ __global__ void __launch_bounds__(256, 2) k_linear_dw(DwArgs a) {
     for (int i = 0; i < 4 * TI; ++i) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
   auto step = [&](auto whole, int64_t r) __attribute__((always_inline)) {
     constexpr bool WHOLE = decltype(whole)::value;
+    constexpr int ES = F32 ? 4 : 1;  // rows from one of a lane's to its next
     Pack<T, 4> vx[TI][RE], vd[RE];
     Pack<Q, 4> vf[RE];
+    const T *p = px + r * a.ldx, *d = pd + r * a.ld_dy;
+    const Q *q = pf + r * a.Co;
 #pragma unroll
     for (int e = 0; e < RE; ++e) {
-      const int64_t row = r + (F32 ? 4 * e : e);
-      const bool in = row + lr < r1;
+      const bool in = r + ES * e + lr < r1;
 #pragma unroll
-      for (int t = 0; t < TI; ++t) {
-        const T *p = px + row * a.ldx + 64 * t;
-        vx[t][e] = WHOLE ? load_pack<T, 4>(p + ox) : load_some<T, 4>(p + ox, in ? a.Ci - ci - 64 * t : 0);
-      }
-      const T *p = pd + row * a.ld_dy;
-      vd[e] = WHOLE ? load_pack<T, 4>(p + od) : load_some<T, 4>(p + od, in ? no : 0);
-      if constexpr (FACTOR != FACTOR_NONE) {
-        const Q *q = pf + row * a.Co;
-        vf[e] = WHOLE ? load_pack<Q, 4>(q + of) : load_some<Q, 4>(q + of, in ? no : 0);
-      }
+      for (int t = 0; t < TI; ++t)
+        vx[t][e] = WHOLE ? load_pack<T, 4>(p + 64 * t + ox) : load_some<T, 4>(p + 64 * t + ox, in ? a.Ci - ci - 64 * t : 0);
+      vd[e] = WHOLE ? load_pack<T, 4>(d + od) : load_some<T, 4>(d + od, in ? no : 0);
+      if constexpr (FACTOR != FACTOR_NONE) vf[e] = WHOLE ? load_pack<Q, 4>(q + of) : load_some<Q, 4>(q + of, in ? no : 0);
+      p += ES * a.ldx;
+      d += ES * a.ld_dy;
+      q += ES * a.Co;
       if (!WHOLE) __builtin_amdgcn_sched_barrier(0);  // (a row at a time: nothing to gain, and fewer registers)
     }
-    if constexpr (FACTOR != FACTOR_NONE)
-#pragma unroll
-      for (int e = 0; e < RE; ++e)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) vd[e].v[j] = (T)((float)vd[e].v[j] * factor_value<FACTOR>(vf[e].v[j], a.leak));
+    auto dz = [&](int e, int j) __attribute__((always_inline)) {
+      float v = (float)vd[e].v[j];
+      if constexpr (FACTOR != FACTOR_NONE) v *= factor_value<FACTOR>(vf[e].v[j], a.leak);
+      return v;
+    };
     if constexpr (F32) {
 #pragma unroll
       for (int e = 0; e < RE; ++e) {
+        floatx4 z;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[j] = dz(e, j);
+        sums += z;
 #pragma unroll
         for (int i = 0; i < 4 * TI; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[i / 4][e].v[i & 3], vd[e].v[j], acc[i][j], 0, 0, 0);
-        if (bias)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sums[j] += vd[e].v[j];
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[i / 4][e].v[i & 3], z[j], acc[i][j], 0, 0, 0);
       }
     } else {
       F fd[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) fd[j][e] = vd[e].v[j];
-      if (bias)  // column sums: a product with ones in row j, so that the four tiles' sums share one result
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          F one;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) one[e] = li == j ? (T)1.f : (T)0.f;
-          sums = mma(one, fd[j], sums);
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (FACTOR == FACTOR_NONE) fd[j][e] = vd[e].v[j];
+          else fd[j][e] = (T)dz(e, j);
         }
+      // column sums: a product with ones in row j, so that the four tiles' sums share one result (made anew in every step: kept, the
+      // four operands cost sixteen registers)
+      int lj = li;
+      asm("" : "+v"(lj));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        F one;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) one[e] = lj == j ? (T)1.f : (T)0.f;
+        sums = mma(one, fd[j], sums);
+      }
 #pragma unroll
       for (int i = 0; i < 4 * TI; ++i) {
         F fx;
@@ -751,10 +757,6 @@ static int by_factor(const void *factor, int act, F &&f) {
   else return f(std::integral_constant<int, std::is_same<T, __bf16>::value ? FACTOR_HALF : FACTOR_FIXED>());
 }
 
-// planes a tile of dW takes of x: 128 read d_y and the factors half as often; with 16-bit features and factors that is more than the
-// registers hold
-template <class T, int FACTOR>
-constexpr bool dw_wide() { return sizeof(T) == 4 || FACTOR == FACTOR_NONE; }
 // row slices of dW: with its 64 x 64 tiles four workgroups a CU (two of the wide ones), no slice below 256 rows
 static int dw_slices(int64_t N, int n_in, int n_out) {
   const int64_t tiles = (int64_t)((n_in + 63) / 64) * ((n_out + 63) / 64);
@@ -904,12 +906,9 @@ int scn_linear_dweight(const void *x, int64_t ldx, const void *d_y, int64_t ld_d
     using T = decltype(t);
     by_factor<T>(factor, act, [&](auto f) {
       constexpr int FACTOR = decltype(f)::value;
-      if constexpr (dw_wide<T, FACTOR>())
-        if (n_in > 64) {
-          dw_launch<T, 2, FACTOR>(a, as_stream(stream));
-          return 0;
-        }
-      dw_launch<T, 1, FACTOR>(a, as_stream(stream));
+      // (128 planes of x a tile: d_y and the factors are read half as often)
+      if (n_in > 64) dw_launch<T, 2, FACTOR>(a, as_stream(stream));
+      else dw_launch<T, 1, FACTOR>(a, as_stream(stream));
       return 0;
     });
     SCN_CHECK_LAUNCH();

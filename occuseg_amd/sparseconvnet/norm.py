@@ -10,12 +10,11 @@ same in training and evaluation, with the activation inside.
 """
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 from torch.nn import Module, Parameter
 
 from .. import SCN
 from . import conv
-from .tensor import SparseConvNetTensor, apply_function, like_empty, optionalTensor, optionalTensorReturn
+from .tensor import SparseConvNetTensor, apply_function, first_order, like_empty, optionalTensor, optionalTensorReturn
 
 
 class _BatchNormFunction(Function):
@@ -135,18 +134,18 @@ class BatchNormLeakyReLU(BatchNormalization):
 class _GroupNormFunction(Function):
     @staticmethod
     def forward(ctx, features, weight, bias, offsets, eps, groups, activation, leakiness):
-        out = like_empty(features)
-        stats = torch.empty(0, dtype=torch.float32, device=features.device)
+        out = torch.empty(features.shape, dtype=features.dtype, device=features.device)
+        stats = torch.empty((offsets.numel() - 1, groups, 2), dtype=torch.float32, device=features.device)
         SCN.GroupNormalization_updateOutput(features, out, stats, offsets, weight, bias, eps, groups, activation, leakiness)
         ctx.args = groups, activation, leakiness
         ctx.save_for_backward(features, weight, bias, offsets, stats)
         return out
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad_output):
         features, weight, bias, offsets, stats = ctx.saved_tensors
-        grad_input = like_empty(grad_output)
+        grad_input = torch.empty(features.shape, dtype=features.dtype, device=features.device)
         grad_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
         grad_bias = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
         SCN.GroupNormalization_backward(features, grad_input, grad_output, stats, offsets, weight, bias, grad_weight, grad_bias,

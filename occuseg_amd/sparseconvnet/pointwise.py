@@ -6,12 +6,15 @@ its kernel.
 """
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 from torch.nn import Module, Parameter
 
 from .. import SCN
 from . import counters
-from .tensor import SparseConvNetTensor, apply_function, like_empty, optionalTensor
+from .tensor import SparseConvNetTensor, apply_function, first_order, optionalTensor
+
+
+def _new(like, *shape):
+    return torch.empty(shape, dtype=like.dtype, device=like.device)
 
 
 def _like(input, features):
@@ -21,17 +24,17 @@ def _like(input, features):
 class _DropoutFunction(Function):
     @staticmethod
     def forward(ctx, features, p, rng):
-        out = like_empty(features)
+        out = _new(features, *features.shape)
         SCN.Dropout_updateOutput(features, out, p, rng)
         ctx.p = p
         ctx.save_for_backward(rng)
         return out
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad_output):
         (rng,) = ctx.saved_tensors
-        grad_input = like_empty(grad_output)
+        grad_input = _new(grad_output, *grad_output.shape)
         SCN.Dropout_updateGradInput(grad_input, grad_output, ctx.p, rng)
         return grad_input, None, None
 
@@ -76,10 +79,11 @@ class Dropout(_Random):
 class _FusedNiNFunction(Function):
     @staticmethod
     def forward(ctx, features, weight, bias, residual, activation, leakiness, p, rng):
-        out = like_empty(features)
+        shape = features.size(0), weight.size(1)
+        out = _new(features, *shape)
         # what the backward pass needs of activation and mask: their common derivative, one value per output
         wanted = any(ctx.needs_input_grad[:3]) and (p > 0 or activation != "leaky_relu" or leakiness != 1)
-        factor = torch.empty(0, dtype=SCN.factor_dtype(features), device=features.device) if wanted else None
+        factor = torch.empty(shape, dtype=SCN.factor_dtype(features), device=features.device) if wanted else None
         macs = SCN.FusedNetworkInNetwork_updateOutput(features, out, weight, bias, residual, activation, leakiness, p, rng, factor)
         counters.add(macs, out.nelement())
         ctx.has_bias, ctx.args = bias.numel() > 0, (activation, leakiness, p)
@@ -87,14 +91,14 @@ class _FusedNiNFunction(Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad_output):
         features, weight, factor = ctx.saved_tensors
         need_x, need_w, need_b, need_res = ctx.needs_input_grad[:4]
         need_b = need_b and ctx.has_bias
-        grad_input = like_empty(grad_output) if need_x else None
-        grad_weight = like_empty(grad_output) if need_w or need_b else None
-        grad_bias = like_empty(grad_output) if need_b else None
+        grad_input = _new(features, *features.shape) if need_x else None
+        grad_weight = _new(weight, *weight.shape) if need_w or need_b else None
+        grad_bias = _new(weight, weight.size(1)) if need_b else None
         if need_x or need_w or need_b:
             SCN.FusedNetworkInNetwork_backward(features, grad_input, grad_output, weight, grad_weight, grad_bias, *ctx.args, factor)
         return (grad_input, grad_weight if need_w else None, grad_bias, grad_output if need_res else None) + (None,) * 4

@@ -3,7 +3,10 @@
 Mirrors sparseconvnet/sparseConvNetTensor.py:13-26, sparseconvnet/metadata.py:16-17 and
 sparseconvnet/utils.py:13-28 (behaviour, not text).
 """
+import functools
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import SCN
 
@@ -216,3 +219,14 @@ def apply_function(fn, *args):
     if torch.is_grad_enabled():
         return fn.apply(*args)
     return fn.forward(_NoGraphCtx(), *args)
+
+
+def first_order(backward):
+    """a Function's backward whose results have no derivatives of their own (once_differentiable, whose bookkeeping is skipped in a
+    pass that records nothing)"""
+    recording = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        return recording(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return wrapper
