@@ -258,6 +258,73 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Few sites: one launch, a workgroup per sample and group that keeps its values in registers.  1024 threads x GN_SMALL_PER values, in
+// row order: a thread's next value is 1024 values on.
+constexpr int GN_SMALL_PER = 32;
+template <class T, int ACT>
+__global__ void __launch_bounds__(1024)
+    k_gn_small(const T *x, T *y, GnArgs a, double eps, float2 *stats, const float *weight, const float *bias) {
+  __shared__ float red[16];
+  const int s = blockIdx.x, g = blockIdx.y;
+  const int64_t start = max(a.offsets[s], (int64_t)0), end = min(a.offsets[s + 1], a.N);
+  const int n = (int)max(end - start, (int64_t)0) * a.cpg;
+  float2 *st = stats + (int64_t)s * a.G + g;
+  if (n == 0) {
+    if (threadIdx.x == 0) *st = make_float2(0.f, 0.f);
+    return;
+  }
+  auto block_sum = [&](float v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if (lane_id() == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) v += red[w];
+    return v;
+  };
+  const int dr = 1024 / a.cpg, dj = 1024 % a.cpg, r0 = (int)threadIdx.x / a.cpg, j0 = (int)threadIdx.x % a.cpg;
+  const int64_t base = start * a.C + g * a.cpg;
+  const T *p = x + base;
+  const float pivot = (float)p[0];
+  float v[GN_SMALL_PER], sum = 0.f, sq = 0.f;
+  int r = r0, j = j0;
+#pragma unroll
+  for (int i = 0; i < GN_SMALL_PER; ++i) {
+    v[i] = 0.f;
+    if (1024 * i < n) {  // (uniform)
+      if (1024 * i + (int)threadIdx.x < n) v[i] = (float)p[(int64_t)r * a.C + j] - pivot;
+      r += dr;
+      j += dj;
+      if (j >= a.cpg) j -= a.cpg, ++r;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < GN_SMALL_PER; ++i) sum += v[i];
+  const float mean = block_sum(sum) / (float)n;  // (of the deviations from the pivot)
+#pragma unroll
+  for (int i = 0; i < GN_SMALL_PER; ++i) {
+    v[i] -= mean;
+    if (1024 * i + (int)threadIdx.x < n) sq = fmaf(v[i], v[i], sq);
+  }
+  const float rstd = (float)(1.0 / sqrt((double)block_sum(sq) / n + eps));
+  if (threadIdx.x == 0) *st = make_float2(pivot + mean, rstd);
+  r = r0, j = j0;
+#pragma unroll
+  for (int i = 0; i < GN_SMALL_PER; ++i) {
+    if (1024 * i >= n) break;
+    if (1024 * i + (int)threadIdx.x < n) {
+      const int c = g * a.cpg + j;
+      y[base + (int64_t)r * a.C + j] =
+          (T)act_value<ACT, sizeof(T) == 4>(fmaf(v[i], rstd * (weight ? weight[c] : 1.f), bias ? bias[c] : 0.f), a.leak);
+    }
+    r += dr;
+    j += dj;
+    if (j >= a.cpg) j -= a.cpg, ++r;
+  }
+}
+
 // ----------------------------------------------------------------- backward ---
 // partial[chunk][plane] = (sum dz, sum dz xh)
 template <class T, int V, int ACT>
@@ -461,6 +528,14 @@ static int gn_forward(const void *x, void *y, float *stats, GnArgs a, const floa
                       void *temp, hipStream_t st) {
   const unsigned chunks = (unsigned)gn_chunks(a);
   float2 *partial = (float2 *)temp;
+  // (a sample has at most N sites: whatever the lengths are, a group's values fit the registers; many samples of a few sites each would
+  // be as many workgroups with next to nothing to do)
+  if (a.N * a.cpg <= 1024 * GN_SMALL_PER && (int64_t)a.S * a.G <= 4096) {
+    auto small = act == SCN_ACT_SILU ? k_gn_small<T, SCN_ACT_SILU> : act == SCN_ACT_GELU ? k_gn_small<T, SCN_ACT_GELU> : k_gn_small<T, SCN_ACT_LEAKY>;
+    small<<<dim3(a.S, a.G), 1024, 0, st>>>((const T *)x, (T *)y, a, eps, (float2 *)stats, weight, bias);
+    SCN_CHECK_LAUNCH();
+    return 0;
+  }
   k_gn_stats<T, V><<<chunks, 256, sizeof(float2) * a.step * V, st>>>((const T *)x, a, partial);
   SCN_CHECK_LAUNCH();
   k_gn_join<<<dim3(a.S, (a.G + JOIN - 1) / JOIN), 1024, 0, st>>>(partial, a, eps, (float2 *)stats);

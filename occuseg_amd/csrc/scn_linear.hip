@@ -17,70 +17,6 @@
 
 namespace scn {
 
-// ------------------------------------------------------------------- dropout ---
-// Every element read and written once; the mask is made of the counter.  A thread keeps its planes -- Q quads -- and walks the
-// sites, `rows` of a step at a time: the products of the counter that belong to the planes are made once.
-template <class T, int Q, bool WHOLE>
-__global__ void __launch_bounds__(256)
-    k_dropout(const T *x, int64_t ldx, T *y, int64_t N, int C, int items, int rows, uint32_t threshold, float scale, const int64_t *rng) {
-  const int item = rows > 1 ? (int)threadIdx.x % items : (int)(blockIdx.y * 256 + threadIdx.x);
-  const int sub = rows > 1 ? (int)threadIdx.x / items : 0;
-  if (item >= items || sub >= rows) return;
-  const RngKey key = rng_key(rng);
-  const int c = item * 4 * Q, n = WHOLE ? 4 * Q : min(4 * Q, C - c);
-  PhiloxPlane plane[Q];
-#pragma unroll
-  for (int u = 0; u < Q; ++u) plane[u] = philox_plane(key, (uint32_t)(item * Q + u));
-  const int64_t step = (int64_t)gridDim.x * rows;
-  for (int64_t row = (int64_t)blockIdx.x * rows + sub; row < N; row += step) {
-    const T *p = x + row * ldx + c;
-    Pack<T, 4 * Q> v;
-    if (n == 4 * Q) v = load_pack<T, 4 * Q>(p);
-    else
-#pragma unroll
-      for (int j = 0; j < 4 * Q; ++j) v.v[j] = j < n ? p[j] : (T)0.f;
-    const PhiloxSite site = philox_site(key, (uint32_t)row);
-#pragma unroll
-    for (int u = 0; u < Q; ++u) {
-      const Words w = philox(key, plane[u], site);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v.v[4 * u + j] = w.w[j] >= threshold ? (T)((float)v.v[4 * u + j] * scale) : (T)0.f;
-    }
-    T *o = y + row * C + c;
-    if (n == 4 * Q) store_pack<T, 4 * Q>(o, v);
-    else
-#pragma unroll
-      for (int j = 0; j < 4 * Q; ++j)
-        if (j < n) o[j] = v.v[j];
-  }
-}
-
-__global__ void k_rng_take(int64_t *state, int64_t *used) {
-  const int64_t seed = state[0], offset = state[1];
-  used[0] = seed;
-  used[1] = offset;
-  state[1] = offset + 1;
-}
-
-// ------------------------------------------------------------------ products ---
-// one k-group = four lane quarters x 16 bytes of a row: 16 fp32 or 32 16-bit values
-template <class T> struct Frag;
-template <> struct Frag<float> { using type = floatx4; };
-template <> struct Frag<__bf16> { using type = bf16x8; };
-template <> struct Frag<_Float16> { using type = halfx8; };
-
-__device__ __forceinline__ floatx4 mma(const floatx4 &a, const floatx4 &b, floatx4 c) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-  return c;
-}
-__device__ __forceinline__ floatx4 mma(const bf16x8 &a, const bf16x8 &b, const floatx4 &c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ floatx4 mma(const halfx8 &a, const halfx8 &b, const floatx4 &c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
 // n of the V elements at p, zeros behind them (16-bit ones packed as they come, or each would keep a register of its own)
 template <class T, int V>
 __device__ __forceinline__ Pack<T, V> load_some(const T *p, int n) {
@@ -109,6 +45,75 @@ __device__ __forceinline__ void store_some(T *p, const Pack<T, V> &v, int n) {
 #pragma unroll
     for (int j = 0; j < V; ++j)
       if (j < n) p[j] = v.v[j];
+}
+
+// ------------------------------------------------------------------- dropout ---
+// Every element read and written once; the mask is made of the counter.  A thread keeps its planes -- Q quads -- and walks the
+// sites, `rows` of a step at a time: the products of the counter that belong to the planes are made once.
+template <class T, int Q, bool WHOLE>
+__global__ void __launch_bounds__(256)
+    k_dropout(const T *x, int64_t ldx, T *y, int64_t N, int C, int items, int rows, uint32_t threshold, float scale, const int64_t *rng) {
+  const int item = rows > 1 ? (int)threadIdx.x % items : (int)(blockIdx.y * 256 + threadIdx.x);
+  const int sub = rows > 1 ? (int)threadIdx.x / items : 0;
+  if (item >= items || sub >= rows) return;
+  const RngKey key = rng_key(rng);
+  const int c = item * 4 * Q, n = WHOLE ? 4 * Q : min(4 * Q, C - c);
+  PhiloxPlane plane[Q];
+#pragma unroll
+  for (int u = 0; u < Q; ++u) plane[u] = philox_plane(key, (uint32_t)(item * Q + u));
+  const int64_t step = (int64_t)gridDim.x * rows;
+  auto masked = [&](Pack<T, 4 * Q> &v, int64_t row) __attribute__((always_inline)) {
+    const PhiloxSite site = philox_site(key, (uint32_t)row);
+#pragma unroll
+    for (int u = 0; u < Q; ++u) {
+      const Words w = philox(key, plane[u], site);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v.v[4 * u + j] = w.w[j] >= threshold ? (T)((float)v.v[4 * u + j] * scale) : (T)0.f;
+    }
+  };
+  int64_t row = (int64_t)blockIdx.x * rows + sub;
+  if (n == 4 * Q)
+    for (; row + 3 * step < N; row += 4 * step) {
+      Pack<T, 4 * Q> v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = load_pack<T, 4 * Q>(x + (row + i * step) * ldx + c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        masked(v[i], row + i * step);
+        store_pack<T, 4 * Q>(y + (row + i * step) * C + c, v[i]);
+      }
+    }
+  for (; row < N; row += step) {
+    Pack<T, 4 * Q> v = load_some<T, 4 * Q>(x + row * ldx + c, n);
+    masked(v, row);
+    store_some<T, 4 * Q>(y + row * C + c, v, n);
+  }
+}
+
+__global__ void k_rng_take(int64_t *state, int64_t *used) {
+  const int64_t seed = state[0], offset = state[1];
+  used[0] = seed;
+  used[1] = offset;
+  state[1] = offset + 1;
+}
+
+// ------------------------------------------------------------------ products ---
+// one k-group = four lane quarters x 16 bytes of a row: 16 fp32 or 32 16-bit values
+template <class T> struct Frag;
+template <> struct Frag<float> { using type = floatx4; };
+template <> struct Frag<__bf16> { using type = bf16x8; };
+template <> struct Frag<_Float16> { using type = halfx8; };
+
+__device__ __forceinline__ floatx4 mma(const floatx4 &a, const floatx4 &b, floatx4 c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ floatx4 mma(const bf16x8 &a, const bf16x8 &b, const floatx4 &c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 mma(const halfx8 &a, const halfx8 &b, const floatx4 &c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 // What the backward pass needs of activation and mask, one value per output: the slope, 0 for a dropped element.  (dy slope is what is
