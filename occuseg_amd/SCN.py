@@ -1914,7 +1914,7 @@ def _rows(t):
     tensor), anything else is copied"""
     if t.is_contiguous():
         return t, t.size(1)
-    if t.stride(1) == 1 and t.stride(0) >= t.size(1):
+    if t.stride(1) == 1 and t.size(1) <= t.stride(0) <= 1 << 26:
         return t, t.stride(0)
     return t.contiguous(), t.size(1)
 

@@ -14,8 +14,6 @@
 // planes, and their constants, for the whole chunk.
 #include "scn_pointwise.h"
 
-#include <type_traits>
-
 namespace scn {
 
 struct GnArgs {
@@ -43,7 +41,7 @@ __device__ __forceinline__ bool gn_chunk(const GnArgs &a, int64_t b, int &s, int
   const int64_t start = max(a.offsets[s], (int64_t)0), end = min(a.offsets[s + 1], a.N);
   r0 = start + ((b - ((start >> a.shift) + s)) << a.shift);
   r1 = min(r0 + ((int64_t)1 << a.shift), end);
-  return r0 < r1;
+  return start <= r0 && r0 < r1;  // (the first: offsets that do not ascend are never followed outside of the tensor)
 }
 
 // f(i, vector) for the thread's vectors of the span [0, span) of p: vector q, q + step, ...; the span's last vector may be partial,
@@ -240,7 +238,6 @@ __global__ void __launch_bounds__(256)
   const int span = (int)(r1 - r0) * a.C;
   const T *p = x + r0 * a.C;
   T *o = y + r0 * a.C;
-  constexpr bool FINE = sizeof(T) == 4;
   for (int q = threadIdx.x; q < a.step; q += 256) {
     float mean[V], w[V], b[V];
     gn_planes<V>(a, q, [&](int j, int c, int gi) {
@@ -252,7 +249,7 @@ __global__ void __launch_bounds__(256)
     gn_walk<4, T, V>(p, span, q, a.step, [&](int i, int n, const Pack<T, V> &v) {
       Pack<T, V> r;
 #pragma unroll
-      for (int j = 0; j < V; ++j) r.v[j] = (T)act_value<ACT, FINE>(fmaf((float)v.v[j] - mean[j], w[j], b[j]), a.leak);
+      for (int j = 0; j < V; ++j) r.v[j] = (T)act_value<ACT, T>(fmaf((float)v.v[j] - mean[j], w[j], b[j]), a.leak);
       gn_store<T, V>(o + i, n, r);
     });
   }
@@ -317,7 +314,7 @@ __global__ void __launch_bounds__(1024)
     if (1024 * i + (int)threadIdx.x < n) {
       const int c = g * a.cpg + j;
       y[base + (int64_t)r * a.C + j] =
-          (T)act_value<ACT, sizeof(T) == 4>(fmaf(v[i], rstd * (weight ? weight[c] : 1.f), bias ? bias[c] : 0.f), a.leak);
+          (T)act_value<ACT, T>(fmaf(v[i], rstd * (weight ? weight[c] : 1.f), bias ? bias[c] : 0.f), a.leak);
     }
     r += dr;
     j += dj;
@@ -336,7 +333,6 @@ __global__ void __launch_bounds__(256)
   if (!gn_chunk(a, blockIdx.x, s, r0, r1)) return;
   const int span = (int)(r1 - r0) * a.C, E = a.step * V;
   const T *p = x + r0 * a.C, *g = dy + r0 * a.C;
-  constexpr bool FINE = sizeof(T) == 4;
   for (int q = threadIdx.x; q < a.step; q += 256) {
     float mean[V], rstd[V], w[V], b[V], s1[V], s2[V];
     gn_planes<V>(a, q, [&](int j, int c, int gi) {
@@ -351,7 +347,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float c = (float)v.v[j] - mean[j];
-        const float dz = j < n ? (float)d.v[j] * act_slope<ACT, FINE>(fmaf(c, w[j], b[j]), a.leak) : 0.f;
+        const float dz = j < n ? (float)d.v[j] * act_slope<ACT, T>(fmaf(c, w[j], b[j]), a.leak) : 0.f;
         s1[j] += dz;
         s2[j] = fmaf(dz, c * rstd[j], s2[j]);
       }
@@ -458,7 +454,6 @@ __global__ void __launch_bounds__(256)
   const int span = (int)(r1 - r0) * a.C;
   const T *p = x + r0 * a.C, *g = dy + r0 * a.C;
   T *o = dx + r0 * a.C;
-  constexpr bool FINE = sizeof(T) == 4;
   for (int q = threadIdx.x; q < a.step; q += 256) {
     float mean[V], w[V], b[V], m1[V], m2[V];
     gn_planes<V>(a, q, [&](int j, int c, int gi) {
@@ -474,7 +469,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float c = (float)v.v[j] - mean[j];
-        const float dz = (float)d.v[j] * act_slope<ACT, FINE>(fmaf(c, w[j], b[j]), a.leak);
+        const float dz = (float)d.v[j] * act_slope<ACT, T>(fmaf(c, w[j], b[j]), a.leak);
         r.v[j] = (T)(fmaf(dz, w[j], -m1[j]) - c * m2[j]);
       }
       gn_store<T, V>(o + i, n, r);

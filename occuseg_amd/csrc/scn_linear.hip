@@ -13,8 +13,6 @@
 // operands (one 16x16x32 of 16-bit types, four 16x16x4 of fp32).  The weights are laid out in LDS in the order of the A operands.
 #include "scn_pointwise.h"
 
-#include <type_traits>
-
 namespace scn {
 
 // n of the V elements at p, zeros behind them (16-bit ones packed as they come, or each would keep a register of its own)
@@ -158,7 +156,7 @@ constexpr int ACT_NONE = 3;  // SCN_ACT_LEAKY with slope 1
 template <class T, int ACT, bool DROP>
 __device__ __forceinline__ float activated(float z, bool keep, const LinearArgs &a, typename FactorOf<T>::type &factor) {
   float value = z, slope = 1.f;
-  if constexpr (ACT != ACT_NONE) act_value_slope<ACT, sizeof(T) == 4>(z, a.leak, value, slope);
+  if constexpr (ACT != ACT_NONE) act_value_slope<ACT, T>(z, a.leak, value, slope);
   if constexpr (DROP) value = keep ? value * a.up : 0.f;
   if constexpr (sizeof(T) == 4) factor = slope;
   else if constexpr (ACT == ACT_NONE) factor = 2;
@@ -174,12 +172,12 @@ constexpr int LIN_ROWS = 128;  // rows of a workgroup's tile: 4 waves x 2 x 16
 constexpr int lin_piece(int nt) { return nt < 4 ? 16 * nt : 64; }  // planes of a tile that go through LDS together
 
 // MODE 0: forward with the epilogue, X its activation.  MODE 1: dx, X how the factors are stored.
-// A workgroup holds the weights of NT x 16 output planes in LDS -- all of K, once, if they fit: then its waves walk 32-row tiles of
-// their own without a barrier -- else `chunk_groups` at a time, and its waves keep together.
+// A workgroup holds the weights of NT x 16 output planes in LDS -- all of K, once, if they fit (STAY): then its waves walk 32-row tiles
+// of their own without a barrier -- else `chunk_groups` at a time, and its waves keep together.
 // Beside fp32 MFMAs a vector instruction costs 8 or more of the matrix pipe's cycles, and the epilogue alone fills half the time of
 // a 16-bit layer: addresses are a scalar base and one 32-bit offset a lane for all tiles, the bias is what the accumulators start
 // from, and the epilogue is compiled for each activation, with and without dropout and factors.
-template <class T, int NT, int MODE, int X>
+template <class T, int NT, int MODE, int X, bool STAY>
 __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
   constexpr int V = Elem<T>::V, KG = 4 * V;
   constexpr int PC = lin_piece(NT), PITCH = PC + 4, LPR = PC / V, RPI = 64 / LPR;  // planes, lanes a row, rows an instruction of a piece
@@ -212,13 +210,12 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
   RngKey key = {};
   if (MODE == 0 && a.threshold) key = rng_key(a.rng);
   const int full = a.K / KG;  // k-groups that lie inside the rows
-  const bool stay = a.groups <= a.chunk_groups;
-  const int tiles = (int)(stay ? (a.N + 31) / 32 : (a.N + LIN_ROWS - 1) / LIN_ROWS * 4);
+  const int tiles = (int)(STAY ? (a.N + 31) / 32 : (a.N + LIN_ROWS - 1) / LIN_ROWS * 4);
 
   // weights of k-groups g0 .. g0 + ng in the order of the A operands, several loads a thread in flight
   auto stage = [&](int g0, int ng) __attribute__((always_inline)) {
     constexpr int B = 4;
-    if (MODE == 1 || NT == 8 || a.transposed) {  // [M, K]: a lane's V elements lie together
+    if (MODE == 1 || NT == 8 || !STAY || a.transposed) {  // [M, K]: a lane's V elements lie together
       for (int e0 = threadIdx.x; e0 < NT * ng * 64; e0 += 256 * B) {
         Pack<T, V> v[B];
 #pragma unroll
@@ -243,7 +240,7 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
       }
     }
   };
-  if (stay) stage(0, a.groups);
+  if (STAY) stage(0, a.groups);
   __syncthreads();
 
   // a piece of results: 16 sites x PC planes from LDS, this lane's V planes of every RPI-th of them.  WHOLE: all of them are there, and
@@ -336,12 +333,10 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[0][t] = acc[1][t] = *(const floatx4 *)(bl + 16 * t + 4 * lq);
 
-    // G k-groups: their rows are requested together (a row's two halves of a cache line one behind the other), then multiplied
-    auto batch = [&](auto count, auto whole, int g, const F *wg) __attribute__((always_inline)) {
-      constexpr int G = decltype(count)::value;
+    // k-groups: the rows of G of them are requested together (a row's two halves of a cache line one behind the other), then multiplied
+    auto request = [&](auto whole, auto &v, auto &f, int g) __attribute__((always_inline)) {
       constexpr bool WHOLE = decltype(whole)::value;
-      Pack<T, V> v[G][2];
-      Pack<Q, V> f[G][2];
+      constexpr int G = sizeof(v) / sizeof(v[0]);
       const T *pk = p + g * KG;
       const Q *pfk = pf + g * KG;
       const int left = a.K - g * KG - lq * V;
@@ -352,6 +347,9 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
           v[i][u] = WHOLE ? load_pack<T, V>(pk + i * KG + op[u]) : load_some<T, V>(pk + i * KG + op[u], left - i * KG);
           if constexpr (FACTORS) f[i][u] = WHOLE ? load_pack<Q, V>(pfk + i * KG + of[u]) : load_some<Q, V>(pfk + i * KG + of[u], left - i * KG);
         }
+    };
+    auto multiply = [&](auto &v, auto &f, const F *wg) __attribute__((always_inline)) {
+      constexpr int G = sizeof(v) / sizeof(v[0]);
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         F b[2], w[NT];
@@ -380,19 +378,25 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
         if (NT == 8) __builtin_amdgcn_sched_barrier(0);  // (one k-group's weights in registers at a time)
       }
     };
+    auto batch = [&](auto count, auto whole, int g, const F *wg) __attribute__((always_inline)) {
+      Pack<T, V> v[decltype(count)::value][2];
+      Pack<Q, V> f[decltype(count)::value][2];
+      request(whole, v, f, g);
+      multiply(v, f, wg);
+    };
+    constexpr int PAIR = NT == 8 && FACTORS && sizeof(T) == 4 ? 1 : 2;  // (as many as the registers allow)
     for (int g0 = 0; g0 < a.groups; g0 += a.chunk_groups) {
       const int ng = min(a.chunk_groups, a.groups - g0), nf = min(ng, full - g0);
-      if (!stay) {
+      const F *wg = wl + lane;
+      int g = 0;
+      if constexpr (!STAY) {
         __syncthreads();
         stage(g0, ng);
         __syncthreads();
       }
-      const F *wg = wl + lane;
-      int g = 0;
-      // (as many as the registers allow)
-      if (NT < 8 && !FACTORS)
+      if (STAY && NT < 8 && !FACTORS)
         for (; g + 4 <= nf; g += 4, wg += 4 * NT * 64) batch(std::integral_constant<int, 4>(), std::true_type(), g0 + g, wg);
-      if (!(NT == 8 && FACTORS && sizeof(T) == 4))
+      if (PAIR == 2)
         for (; g + 2 <= nf; g += 2, wg += 2 * NT * 64) batch(std::integral_constant<int, 2>(), std::true_type(), g0 + g, wg);
       for (; g < nf; ++g, wg += NT * 64) batch(std::integral_constant<int, 1>(), std::true_type(), g0 + g, wg);
       if (g < ng) batch(std::integral_constant<int, 1>(), std::false_type(), g0 + g, wg);
@@ -594,20 +598,10 @@ __global__ void __launch_bounds__(256, 2) k_linear_dw(DwArgs a) {
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if constexpr (FACTOR == FACTOR_NONE) fd[j][e] = vd[e].v[j];
-          else fd[j][e] = (T)dz(e, j);
+          const float z = dz(e, j);
+          sums[j] += z;  // (of the values that the matrix units' operand rounds)
+          fd[j][e] = (T)z;
         }
-      // column sums: a product with ones in row j, so that the four tiles' sums share one result (made anew in every step: kept, the
-      // four operands cost sixteen registers)
-      int lj = li;
-      asm("" : "+v"(lj));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        F one;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) one[e] = lj == j ? (T)1.f : (T)0.f;
-        sums = mma(one, fd[j], sums);
-      }
 #pragma unroll
       for (int i = 0; i < 4 * TI; ++i) {
         F fx;
@@ -621,13 +615,12 @@ __global__ void __launch_bounds__(256, 2) k_linear_dw(DwArgs a) {
   int64_t r = r0 + wave * ROWS;
   for (; r + ROWS <= inside; r += 4 * ROWS) step(std::true_type(), r);
   for (; r < r1; r += 4 * ROWS) step(std::false_type(), r);
-  // sums[j] of column 4 li + j: fp32 has parts of it in the four lane quarters, 16-bit types all of it in the first
-  if (F32)
+  // sums[j] of column 4 li + j: the four lane quarters' rows
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      sums[j] += __shfl_xor(sums[j], 16);
-      sums[j] += __shfl_xor(sums[j], 32);
-    }
+  for (int j = 0; j < 4; ++j) {
+    sums[j] += __shfl_xor(sums[j], 16);
+    sums[j] += __shfl_xor(sums[j], 32);
+  }
   // waves 1, 2, 3 hand over to wave 0, one after the other
 #pragma unroll 1
   for (int w = 1; w < 4; ++w) {
@@ -692,6 +685,7 @@ __global__ void __launch_bounds__(1024) k_linear_dw_join(const float *slab, int 
 }
 
 // ---------------------------------------------------------------------- host ---
+constexpr int64_t LIN_MAX_LD = (int64_t)1 << 26;  // (31 rows of it in 32 bits)
 static int lin_check(int64_t N, int n_in, int n_out, int dtype) {
   SCN_REQUIRE(dtype == SCN_F32 || dtype == SCN_BF16 || dtype == SCN_F16, "linear: dtype");
   SCN_REQUIRE(n_in >= 1 && n_out >= 1 && n_in <= 65536 && n_out <= 65536, "linear: 1 to 65536 planes");
@@ -704,6 +698,15 @@ static int by_type(int dtype, F &&f) {
   if (dtype == SCN_F32) return f((float)0);
   if (dtype == SCN_BF16) return f((__bf16)0);
   return f((_Float16)0);
+}
+
+// A launch that lays the weights out as [n_out, n_in] costs 2 to 4 us; every workgroup then fetches them by 16 bytes of a reduction
+// instead of by single values.  It pays for itself from some thousand sites on (177,001 x 128 to 512, bf16: 70 to 49 us without an
+// activation), and where the weights do not stay in LDS and every workgroup fetches all of them (four column tiles of 11 k-groups do).
+constexpr int64_t LIN_TRANSPOSE_ROWS = 4096;
+constexpr int LIN_FEW = 4;  // up to this many sites: k_linear_few
+static bool lin_transposes(int64_t N, int n_in, int dtype) {
+  return N > LIN_FEW && (N >= LIN_TRANSPOSE_ROWS || n_in * (dtype == SCN_F32 ? 4 : 2) > 11 * 64);
 }
 
 template <class T, int NT, int MODE, int X>
@@ -722,8 +725,10 @@ static int linear_launch(LinearArgs a, hipStream_t st) {
   int64_t rows = 256 * fit / a.col_blocks / 8 * 8;
   if (rows < 8) rows = 8;
   if (a.groups > a.chunk_groups || rows > tiles) rows = tiles;
+  SCN_REQUIRE(rows * a.col_blocks < ((int64_t)1 << 31), "linear: sites x planes beyond a launch");
   a.row_blocks = (int)rows;
-  k_linear<T, NT, MODE, X><<<(unsigned)(rows * a.col_blocks), 256, lds, st>>>(a);
+  auto k = a.groups <= a.chunk_groups ? k_linear<T, NT, MODE, X, true> : k_linear<T, NT, MODE, X, false>;
+  k<<<(unsigned)(rows * a.col_blocks), 256, lds, st>>>(a);
   SCN_CHECK_LAUNCH();
   return 0;
 }
@@ -739,17 +744,13 @@ static int linear_by_width(const LinearArgs &a, hipStream_t st) {
 }
 template <class T, int ACT>
 static int linear_forward(const LinearArgs &a, hipStream_t st) {
-  if (a.N > 4) return linear_by_width<T, 0, ACT>(a, st);
+  if (a.N > LIN_FEW) return linear_by_width<T, 0, ACT>(a, st);
   const unsigned blocks = (unsigned)((a.M + 15) / 16);
   if (a.N == 1) k_linear_few<T, 1, ACT><<<blocks, 1024, 0, st>>>(a);
   else k_linear_few<T, 4, ACT><<<blocks, 1024, 0, st>>>(a);
   SCN_CHECK_LAUNCH();
   return 0;
 }
-
-// From this many sites on a launch that lays the weights out as [n_out, n_in] pays for itself (2 us; every workgroup then fetches them
-// by 16 bytes of a reduction instead of by single values)
-constexpr int64_t LIN_TRANSPOSE_ROWS = 4096;
 
 // 1 / (1 - p); without factors the pass had no dropout
 static float keep_scale(const void *factor, double p) { return factor ? (float)(1.0 / (1.0 - p)) : 1.f; }
@@ -787,7 +788,7 @@ int scn_dropout(const void *x, int64_t ldx, void *y, int64_t N, int planes, int 
   if (int e = lin_check(N, planes, 1, dtype)) return e;
   SCN_REQUIRE(p >= 0 && p < 1, "dropout: 0 <= p < 1");
   if (N == 0) return 0;
-  SCN_REQUIRE(x && y && rng && ldx >= planes, "dropout: pointers");
+  SCN_REQUIRE(x && y && rng && ldx >= planes, "dropout: pointers and strides");
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int Q = Elem<T>::V / 4;
@@ -811,7 +812,7 @@ int scn_rng_take(int64_t *state, int64_t *used, void *stream) {
 }
 
 size_t scn_linear_forward_temp_bytes(int64_t N, int n_in, int n_out, int dtype) {
-  return N < LIN_TRANSPOSE_ROWS ? 0 : (size_t)n_in * n_out * (dtype == SCN_F32 ? 4 : 2);
+  return lin_transposes(N, n_in, dtype) ? (size_t)n_in * n_out * (dtype == SCN_F32 ? 4 : 2) : 0;
 }
 
 int scn_linear_forward(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_res,
@@ -821,7 +822,8 @@ int scn_linear_forward(const void *x, int64_t ldx, const void *weight, const voi
   SCN_REQUIRE(act == SCN_ACT_LEAKY || act == SCN_ACT_SILU || act == SCN_ACT_GELU, "linear: activation");
   SCN_REQUIRE(p >= 0 && p < 1 && (p == 0 || rng), "linear: 0 <= p < 1, with random words if it is not 0");
   if (N == 0) return 0;
-  SCN_REQUIRE(x && weight && y && ldx >= n_in && (!residual || ld_res >= n_out), "linear: pointers");
+  SCN_REQUIRE(x && weight && y && ldx >= n_in && ldx <= LIN_MAX_LD && (!residual || (ld_res >= n_out && ld_res <= LIN_MAX_LD)),
+              "linear: pointers and strides");
   LinearArgs a = {};
   a.in = x;
   a.ld_in = ldx;
@@ -838,7 +840,7 @@ int scn_linear_forward(const void *x, int64_t ldx, const void *weight, const voi
   a.threshold = drop_threshold(p);
   a.leak = (float)leakiness;
   a.up = (float)(1.0 / (1.0 - p));
-  const bool transpose = N >= LIN_TRANSPOSE_ROWS;
+  const bool transpose = lin_transposes(N, n_in, dtype);
   SCN_REQUIRE(!transpose || (temp && temp_bytes >= scn_linear_forward_temp_bytes(N, n_in, n_out, dtype)), "linear: workspace");
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -861,7 +863,7 @@ int scn_linear_dinput(const void *d_y, int64_t ld_dy, const void *factor, const 
   if (int e = lin_check(N, n_in, n_out, dtype)) return e;
   SCN_REQUIRE(p >= 0 && p < 1, "linear: 0 <= p < 1");
   if (N == 0) return 0;
-  SCN_REQUIRE(d_y && weight && d_x && ld_dy >= n_out, "linear: pointers");
+  SCN_REQUIRE(d_y && weight && d_x && ld_dy >= n_out && ld_dy <= LIN_MAX_LD, "linear: pointers and strides");
   LinearArgs a = {};
   a.in = d_y;
   a.ld_in = ld_dy;
@@ -888,7 +890,8 @@ int scn_linear_dweight(const void *x, int64_t ldx, const void *d_y, int64_t ld_d
                        size_t temp_bytes, void *stream) {
   if (int e = lin_check(N, n_in, n_out, dtype)) return e;
   SCN_REQUIRE(p >= 0 && p < 1, "linear: 0 <= p < 1");
-  SCN_REQUIRE(d_weight && (N == 0 || (x && d_y)) && ldx >= n_in && ld_dy >= n_out, "linear: pointers");
+  SCN_REQUIRE(d_weight && (N == 0 || (x && d_y)) && ldx >= n_in && ld_dy >= n_out && ldx <= LIN_MAX_LD && ld_dy <= LIN_MAX_LD,
+              "linear: pointers and strides");
   SCN_REQUIRE(temp && temp_bytes >= scn_linear_dweight_temp_bytes(N, n_in, n_out), "linear: workspace");
   DwArgs a = {};
   a.x = x;

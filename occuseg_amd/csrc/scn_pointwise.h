@@ -3,6 +3,8 @@
 #pragma once
 #include "scn_common.h"
 
+#include <type_traits>
+
 namespace scn {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -37,12 +39,14 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r) {
 //      SCN_ACT_SILU   z / (1 + e^-z)
 //      SCN_ACT_GELU   z Phi(z), Phi the normal distribution function
 // One reciprocal and one exponential of the hardware each (1 ulp; an exponent x is off by |x| 2^-24, where e^x is as small).  The tail
-// 1 - Phi(t), t >= 0, is e^(-t^2 / 2) times a smooth function of t, here a polynomial in s = 1 / (1 + c t) without a constant term,
-// fitted to erfcx(t / sqrt 2) / 2 over t <= 40 by iteratively reweighted least squares.  Largest relative error of z Phi(z) in fp32 over
-// |z| <= 9: 4.5e-7 with nine terms (FINE, float features), 2.9e-6 with seven (16-bit features: 2^-12 at the finest).
+// 1 - Phi(t), t >= 0, is the density phi(t) -- which the slope needs too -- times a smooth function of t, here a polynomial in
+// s = 1 / (1 + c t) without a constant term, fitted to (1 - Phi) / phi over t <= 40 by iteratively reweighted least squares.  Largest
+// relative error of z Phi(z) over |z| <= 9, in fp32: 4.8e-7 with nine terms (float features), 2.9e-6 with seven (fp16, whose half
+// step is 4.9e-4 at its finest), 6.1e-5 with five (bf16: 3.9e-3).
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+template <class T> constexpr int act_terms() { return sizeof(T) == 4 ? 9 : std::is_same<T, __bf16>::value ? 5 : 7; }
 
-template <int ACT, bool FINE>
+template <int ACT, class T>
 __device__ __forceinline__ void act_value_slope(float z, float leak, float &value, float &slope) {
   if (ACT == SCN_ACT_LEAKY) {
     slope = z > 0 ? 1.f : leak;
@@ -52,42 +56,48 @@ __device__ __forceinline__ void act_value_slope(float z, float leak, float &valu
     value = z * s;
     slope = fmaf(value, 1.f - s, s);
   } else {
-    const float e = exp2_hw(z * z * -0.72134752f), t = fabsf(z);
+    const float dens = exp2_hw(fmaf(z * z, -0.72134752f, -1.32574806f)), t = fabsf(z);
     float p;
-    if (FINE) {
+    if (act_terms<T>() == 9) {
       const float s = __builtin_amdgcn_rcpf(fmaf(0.36f, t, 1.f));
-      p = fmaf(s, -0.030251468f, 0.139558294f);
-      p = fmaf(s, p, -0.223676858f);
-      p = fmaf(s, p, 0.107432581f);
-      p = fmaf(s, p, -0.000416137f);
-      p = fmaf(s, p, 0.096045419f);
-      p = fmaf(s, p, 0.124008544f);
-      p = fmaf(s, p, 0.143681972f);
-      p = fmaf(s, p, 0.143617662f) * s;
-    } else {
+      p = fmaf(s, -0.075829186f, 0.349820765f);
+      p = fmaf(s, p, -0.560674736f);
+      p = fmaf(s, p, 0.269293545f);
+      p = fmaf(s, p, -0.001043101f);
+      p = fmaf(s, p, 0.240750164f);
+      p = fmaf(s, p, 0.310843324f);
+      p = fmaf(s, p, 0.360157293f);
+      p = fmaf(s, p, 0.359996093f) * s;
+    } else if (act_terms<T>() == 7) {
       const float s = __builtin_amdgcn_rcpf(fmaf(0.38f, t, 1.f));
-      p = fmaf(s, 0.048951976f, -0.160032814f);
-      p = fmaf(s, p, 0.114400200f);
-      p = fmaf(s, p, 0.059983662f);
-      p = fmaf(s, p, 0.133793775f);
-      p = fmaf(s, p, 0.151298799f);
-      p = fmaf(s, p, 0.151605686f) * s;
+      p = fmaf(s, 0.122704407f, -0.401142778f);
+      p = fmaf(s, p, 0.286758777f);
+      p = fmaf(s, p, 0.150356744f);
+      p = fmaf(s, p, 0.335371260f);
+      p = fmaf(s, p, 0.379249847f);
+      p = fmaf(s, p, 0.380019100f) * s;
+    } else {
+      const float s = __builtin_amdgcn_rcpf(fmaf(0.39f, t, 1.f));
+      p = fmaf(s, -0.218651797f, 0.413951101f);
+      p = fmaf(s, p, 0.270861309f);
+      p = fmaf(s, p, 0.397368879f);
+      p = fmaf(s, p, 0.389709251f) * s;
     }
-    const float tail = p * e, cdf = z > 0 ? 1.f - tail : tail;
+    const float tail = p * dens, cdf = z > 0 ? 1.f - tail : tail;
     value = z * cdf;
-    slope = fmaf(z * 0.39894228f, e, cdf);
+    slope = fmaf(z, dens, cdf);
   }
 }
-template <int ACT, bool FINE>
+template <int ACT, class T>
 __device__ __forceinline__ float act_value(float z, float leak) {
   float v, s;
-  act_value_slope<ACT, FINE>(z, leak, v, s);
+  act_value_slope<ACT, T>(z, leak, v, s);
   return v;
 }
-template <int ACT, bool FINE>
+template <int ACT, class T>
 __device__ __forceinline__ float act_slope(float z, float leak) {
   float v, s;
-  act_value_slope<ACT, FINE>(z, leak, v, s);
+  act_value_slope<ACT, T>(z, leak, v, s);
   return s;
 }
 
