@@ -26,18 +26,18 @@ struct GnArgs {
   float leak;
 };
 
-// the sample and the rows of chunk b; false: an empty chunk.  Every wave finds it by itself, 64 samples a step.
+// the sample and the rows of chunk b; false: an empty chunk.  Every wave finds it by itself, 64 samples a look: one look for up to 64
+// samples, three for 65535.
 __device__ __forceinline__ bool gn_chunk(const GnArgs &a, int64_t b, int &s, int64_t &r0, int64_t &r1) {
-  int below = 0;
-  for (int base = 0; base < a.S; base += 64) {
-    const int i = base + lane_id();
-    const bool in = i < a.S && (a.offsets[min(i, a.S - 1)] >> a.shift) + i <= b;
-    const int n = __popcll(__ballot(in));
-    below += n;
-    if (n < 64) break;
+  s = 0;
+  for (int hi = a.S;;) {  // the sample looked for is in s .. hi - 1
+    const int step = (hi - s + 63) >> 6, i = s + lane_id() * step;
+    const int n = __popcll(__ballot(i < hi && (a.offsets[min(i, a.S - 1)] >> a.shift) + i <= b));
+    if (n == 0) return false;
+    s += (n - 1) * step;
+    if (step == 1) break;
+    hi = min(hi, s + step);
   }
-  if (below == 0) return false;
-  s = below - 1;
   const int64_t start = max(a.offsets[s], (int64_t)0), end = min(a.offsets[s + 1], a.N);
   r0 = start + ((b - ((start >> a.shift) + s)) << a.shift);
   r1 = min(r0 + ((int64_t)1 << a.shift), end);
@@ -45,7 +45,7 @@ __device__ __forceinline__ bool gn_chunk(const GnArgs &a, int64_t b, int &s, int
 }
 
 // f(i, vector) for the thread's vectors of the span [0, span) of p: vector q, q + step, ...; the span's last vector may be partial,
-// its missing elements are `fill`.
+// its missing elements are zeros.
 template <int UNROLL, class T, int V, class F>
 __device__ __forceinline__ void gn_walk(const T *p, int span, int q, int step, F &&f) {
   int i = q * V;

@@ -157,6 +157,16 @@ def test_group_norm_rows_outside_the_samples_are_left(gpu):
     assert (dx[:7] == 5).all() and (dx[41:] == 5).all() and torch.equal(db, torch.full_like(db, 34))
 
 
+@pytest.mark.parametrize("samples", [300, 5000])
+def test_group_norm_many_samples(gpu, samples):
+    lengths = [(7 * s) % 5 % 4 for s in range(samples)]  # 0 to 3 sites each
+    lengths[samples // 2] = 1500
+    n = sum(lengths)
+    x, dy, w, b = rnd(31, n, 24).float(), rnd(32, n, 24).float(), rnd(33, 24).float().double(), rnd(34, 24).float().double()
+    args = (x, lengths, 2, w, b, 1e-2, "silu", 1.0, dy)
+    check_group_norm(run_group_norm(gpu, *args), *args, "%d samples" % samples)
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_group_norm_bad_values_stay_in_their_group(gpu, bad):
     x = rnd(1, 60, 8).float()
