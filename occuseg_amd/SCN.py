@@ -1931,8 +1931,10 @@ def _opt(t):
     return t if t is not None and t.numel() else None
 
 
-def _sized(t, *shape):
+def _sized(t, dtype, device, *shape):
     """callers pass empty outputs which are resized here, or outputs of the right shape"""
+    if t.dtype is not dtype or t.get_device() != device:
+        raise RuntimeError("occuseg_amd.SCN: a %s output on %s where the kernel writes %s on GPU %d" % (t.dtype, t.device, dtype, device))
     if t.shape != shape:
         t.resize_(*shape)
     elif not t.is_contiguous():
@@ -1977,11 +1979,11 @@ def GroupNormalization_updateOutput(input_features, output_features, stats, offs
     ``stats`` receives (mean, 1 / sqrt(var + eps)) as float32 [samples, groups, 2], which the backward pass takes."""
     what = "GroupNormalization_updateOutput"
     code, N, C, groups, S, act, weight, bias = _group_norm_args(what, input_features, offsets, weight, bias, groups, activation)
-    x = input_features.contiguous()
+    x, device = input_features.contiguous(), input_features.get_device()
     lib = _lib_()
     with _on(x):
-        _sized(output_features, N, C)
-        _sized(stats, S, groups, 2)
+        _sized(output_features, x.dtype, device, N, C)
+        _sized(stats, torch.float32, device, S, groups, 2)
         tb = lib.scn_group_norm_temp_bytes(N, C, groups, S, code, 0)
         temp = torch.empty(tb, dtype=torch.uint8, device=x.device)
         ev = _prof_begin("bn")
@@ -1997,17 +1999,23 @@ def GroupNormalization_backward(input_features, d_input_features, d_output_featu
     what = "GroupNormalization_backward"
     code, N, C, groups, S, act, weight, bias = _group_norm_args(what, input_features, offsets, weight, bias, groups, activation)
     _pointwise(what, d_output_features, input_features)
-    if d_output_features.shape != input_features.shape or stats.numel() != 2 * S * groups or stats.dtype != torch.float32:
+    device = input_features.get_device()
+    if d_output_features.shape != input_features.shape or stats.shape != (S, groups, 2):
         raise RuntimeError("occuseg_amd.SCN.%s: shapes" % what)
+    d_weight, d_bias = _opt(d_weight), _opt(d_bias)
     x, dy = input_features.contiguous(), d_output_features.contiguous()
     lib = _lib_()
     with _on(x):
-        _sized(d_input_features, N, C)
+        _sized(d_input_features, x.dtype, device, N, C)
+        _sized(stats, torch.float32, device, S, groups, 2)
+        for t in (d_weight, d_bias):
+            if t is not None:
+                _sized(t, torch.float32, device, C)
         tb = lib.scn_group_norm_temp_bytes(N, C, groups, S, code, 1)
         temp = torch.empty(tb, dtype=torch.uint8, device=x.device)
         ev = _prof_begin("bn")
         check(lib.scn_group_norm_backward(ptr(x), ptr(dy), ptr(d_input_features), ptr(stats), ptr(offsets), ptr(weight),
-                                          ptr(bias), ptr(_opt(d_weight)), ptr(_opt(d_bias)), act, float(leakiness), N, C, groups,
+                                          ptr(bias), ptr(d_weight), ptr(d_bias), act, float(leakiness), N, C, groups,
                                           S, code, ptr(temp), tb, stream()))
         if ev is not None:
             _prof_end(ev, "gn_bwd", 0.0, 5.0 * N * C * x.element_size(), (N, C, groups))
@@ -2022,7 +2030,7 @@ def Dropout_updateOutput(input_features, output_features, p, rng):
     x, ld = _rows(input_features)
     N, C = x.shape
     with _on(x):
-        _sized(output_features, N, C)
+        _sized(output_features, x.dtype, x.get_device(), N, C)
         if C:
             check(_lib_().scn_dropout(ptr(x), ld, ptr(output_features), N, C, code, p, ptr(rng), stream()))
 
@@ -2076,14 +2084,12 @@ def FusedNetworkInNetwork_updateOutput(input_features, output_features, weight, 
         if residual.shape != (N, Co):
             raise RuntimeError("occuseg_amd.SCN.%s: residual %s for an output of %s" % (what, tuple(residual.shape), (N, Co)))
         res, ld_res = _rows(residual)
-    if factor is not None and (factor.dtype is not factor_dtype(x) or factor.get_device() != x.get_device()):
-        raise RuntimeError("occuseg_amd.SCN.%s: factor must be %s" % (what, factor_dtype(x)))
     weight = weight.contiguous()
     lib = _lib_()
     with _on(x):
-        _sized(output_features, N, Co)
+        _sized(output_features, x.dtype, x.get_device(), N, Co)
         if factor is not None:
-            _sized(factor, N, Co)
+            _sized(factor, factor_dtype(x), x.get_device(), N, Co)
         tb = lib.scn_linear_forward_temp_bytes(N, Ci, Co, code)
         temp = torch.empty(tb, dtype=torch.uint8, device=x.device) if tb else None
         ev = _prof_begin()
@@ -2114,15 +2120,15 @@ def FusedNetworkInNetwork_backward(input_features, d_input_features, d_output_fe
         nbytes = float(x.element_size()) * (N * (Ci + Co * (1 + (factor is not None))) + Ci * Co) if PROFILE is not None else 0.0
         if d_input_features is not None:
             weight = weight.contiguous()
-            _sized(d_input_features, N, Ci)
+            _sized(d_input_features, x.dtype, x.get_device(), N, Ci)
             ev = _prof_begin()
             check(lib.scn_linear_dinput(ptr(dy), ld_dy, ptr(factor), ptr(weight), ptr(d_input_features), N, Ci, Co, act,
                                         leakiness, p, code, stream()))
             _prof_end(ev, "linear_dx", 2.0 * N * Ci * Co, nbytes, (N, Ci, Co))
         if d_weight is not None:
-            _sized(d_weight, Ci, Co)
+            _sized(d_weight, x.dtype, x.get_device(), Ci, Co)
             if d_bias is not None:
-                _sized(d_bias, Co)
+                _sized(d_bias, x.dtype, x.get_device(), Co)
             tb = lib.scn_linear_dweight_temp_bytes(N, Ci, Co)
             temp = torch.empty(tb, dtype=torch.uint8, device=x.device)
             ev = _prof_begin()

@@ -545,3 +545,27 @@ def test_refusals(gpu):
     (g,) = torch.autograd.grad(y.sum(), [xg], create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()  # no second derivatives
+
+
+def test_outputs_of_another_type_or_device_are_refused(gpu):
+    """an output that is smaller than what the kernel writes"""
+    from occuseg_amd import SCN
+    x, w, rng = torch.zeros(6, 8, device=gpu), torch.zeros(8, 4, device=gpu), torch.zeros(2, dtype=torch.int64, device=gpu)
+    offsets = torch.tensor([0, 6], device=gpu)
+    e, half, host = x.new_empty(0), x.new_empty(0).half(), torch.empty(0)
+    stats = torch.zeros(1, 2, 2, device=gpu)
+    for bad in (half, host):
+        for call in (lambda: SCN.Dropout_updateOutput(x, bad, 0.5, rng),
+                     lambda: SCN.GroupNormalization_updateOutput(x, bad, e, offsets, None, None, 1e-4, 2, "silu", 1),
+                     lambda: SCN.GroupNormalization_updateOutput(x, e, bad, offsets, None, None, 1e-4, 2, "silu", 1),
+                     lambda: SCN.GroupNormalization_backward(x, bad, x, stats, offsets, None, None, None, None, 2, "silu", 1),
+                     lambda: SCN.GroupNormalization_backward(x, e, x, stats.to(bad), offsets, None, None, None, None, 2, "silu", 1),
+                     lambda: SCN.GroupNormalization_backward(x, e, x, stats, offsets, None, None, torch.zeros(8).to(bad), None, 2, "silu", 1),
+                     lambda: SCN.GroupNormalization_backward(x, e, x, stats, offsets, None, None, None, torch.zeros(8).to(bad), 2, "silu", 1),
+                     lambda: SCN.FusedNetworkInNetwork_updateOutput(x, bad, w, None, None, "silu", 1, 0.0, None),
+                     lambda: SCN.FusedNetworkInNetwork_updateOutput(x, e, w, None, None, "silu", 1, 0.0, None, bad),
+                     lambda: SCN.FusedNetworkInNetwork_backward(x, bad, x[:, :4], w, None, None, "leaky_relu", 1, 0.0),
+                     lambda: SCN.FusedNetworkInNetwork_backward(x, None, x[:, :4], w, bad, None, "leaky_relu", 1, 0.0),
+                     lambda: SCN.FusedNetworkInNetwork_backward(x, None, x[:, :4], w, x.new_empty(0), bad, "leaky_relu", 1, 0.0)):
+            with pytest.raises(RuntimeError, match="output on"):
+                call()
