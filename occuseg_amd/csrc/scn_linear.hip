@@ -689,6 +689,7 @@ constexpr int64_t LIN_MAX_LD = (int64_t)1 << 26;  // (31 rows of it in 32 bits)
 static int lin_check(int64_t N, int n_in, int n_out, int dtype) {
   SCN_REQUIRE(dtype == SCN_F32 || dtype == SCN_BF16 || dtype == SCN_F16, "linear: dtype");
   SCN_REQUIRE(n_in >= 1 && n_out >= 1 && n_in <= 65536 && n_out <= 65536, "linear: 1 to 65536 planes");
+  SCN_REQUIRE((int64_t)n_in * n_out <= ((int64_t)1 << 27), "linear: at most 2^27 weights");  // (16 threads each, of 2^32 a launch)
   SCN_REQUIRE(N >= 0 && N < ((int64_t)1 << 31), "linear: fewer than 2^31 sites");
   return 0;
 }
@@ -725,7 +726,7 @@ static int linear_launch(LinearArgs a, hipStream_t st) {
   int64_t rows = 256 * fit / a.col_blocks / 8 * 8;
   if (rows < 8) rows = 8;
   if (a.groups > a.chunk_groups || rows > tiles) rows = tiles;
-  SCN_REQUIRE(rows * a.col_blocks < ((int64_t)1 << 31), "linear: sites x planes beyond a launch");
+  SCN_REQUIRE(rows * a.col_blocks < ((int64_t)1 << 24), "linear: sites x planes beyond a launch of 2^32 threads");
   a.row_blocks = (int)rows;
   auto k = a.groups <= a.chunk_groups ? k_linear<T, NT, MODE, X, true> : k_linear<T, NT, MODE, X, false>;
   k<<<(unsigned)(rows * a.col_blocks), 256, lds, st>>>(a);

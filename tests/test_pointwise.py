@@ -101,3 +101,21 @@ def test_dropout_state():
     b.reseed(7, 9)
     assert b.rng_state.tolist() == [7, 9]
     assert a.to(torch.bfloat16).rng_state.dtype == torch.int64
+
+
+def test_boundary_refuses_sizes_beyond_a_launch():
+    """the pointers are not looked at: sizes and strides are refused first, on the host"""
+    from occuseg_amd import _lib
+    lib = _lib.load()
+    p = torch.zeros(4).data_ptr()
+    # strides whose multiples leave 32 bits, weights of more than 2^32 threads, sites beyond 2^31
+    assert lib.scn_linear_forward(p, 1 << 27, p, None, None, 0, p, None, 40, 8, 4, 0, 1.0, 0.0, None, 0, None, 0, None) == 2
+    assert lib.scn_linear_forward(p, 8, p, None, p, 1 << 27, p, None, 40, 8, 4, 0, 1.0, 0.0, None, 0, None, 0, None) == 2
+    assert lib.scn_linear_dinput(p, 1 << 27, None, p, p, 40, 8, 4, 0, 1.0, 0.0, 0, None) == 2
+    for ldx, ld_dy in ((1 << 27, 4), (8, 1 << 27)):
+        assert lib.scn_linear_dweight(p, ldx, p, ld_dy, None, p, None, 40, 8, 4, 0, 1.0, 0.0, 0, p, 1 << 40, None) == 2
+    assert lib.scn_linear_dweight(p, 1 << 15, p, 1 << 15, None, p, None, 40, 1 << 15, 1 << 15, 0, 1.0, 0.0, 0, p, 1 << 40, None) == 2
+    assert lib.scn_linear_forward(p, 8, p, None, None, 0, p, None, 1 << 31, 8, 4, 0, 1.0, 0.0, None, 0, p, 1 << 40, None) == 2
+    assert lib.scn_dropout(p, 8, p, 1 << 31, 8, 0, 0.5, p, None) == 2
+    assert lib.scn_dropout(p, 7, p, 40, 8, 0, 0.5, p, None) == 2
+    assert lib.scn_group_norm_temp_bytes(1 << 31, 8, 2, 1, 0, 0) == 0 and lib.scn_group_norm_temp_bytes(10, 8, 2, 1 << 16, 0, 0) == 0
