@@ -42,7 +42,13 @@ class _DropoutFunction(Function):
 class _Random(Module):
     """a module that draws: the buffer `rng_state` = (seed, offset), int64 [2].  The seed comes from torch's CPU generator when the
     module is made; every training forward pass uses one offset.  The counting happens on the device, so a pass captured into a
-    graph draws a new mask at every replay.  Ranks of a data-parallel job that are seeded alike draw alike: `reseed` them."""
+    graph draws a new mask at every replay.  Ranks of a data-parallel job that are seeded alike draw alike: `reseed` them.  A forward
+    pass that is run again for its gradients (activation checkpointing) draws again: hand it `rng`.  A state_dict without the
+    buffer (of a NetworkInNetwork) leaves it as it is."""
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        state_dict.setdefault(prefix + "rng_state", self.rng_state)
+        Module._load_from_state_dict(self, state_dict, prefix, *args)
 
     def _init_rng(self):
         self.register_buffer("rng_state", torch.stack([torch.randint(-2 ** 63, 2 ** 63 - 1, ()), torch.zeros((), dtype=torch.int64)]))

@@ -119,3 +119,14 @@ def test_boundary_refuses_sizes_beyond_a_launch():
     assert lib.scn_dropout(p, 8, p, 1 << 31, 8, 0, 0.5, p, None) == 2
     assert lib.scn_dropout(p, 7, p, 40, 8, 0, 0.5, p, None) == 2
     assert lib.scn_group_norm_temp_bytes(1 << 31, 8, 2, 1, 0, 0) == 0 and lib.scn_group_norm_temp_bytes(10, 8, 2, 1 << 16, 0, 0) == 0
+
+
+def test_fused_layer_takes_the_parameters_of_a_plain_one():
+    import occuseg_amd.sparseconvnet as scn
+    plain, fused = scn.NetworkInNetwork(5, 3, True), scn.FusedNetworkInNetwork(5, 3, True, "silu", dropout=0.1)
+    fused.reseed(3, 4)
+    torch.nn.Sequential(fused).load_state_dict(torch.nn.Sequential(plain).state_dict())
+    assert torch.equal(fused.weight, plain.weight) and fused.rng_state.tolist() == [3, 4]
+    other = scn.FusedNetworkInNetwork(5, 3, True, "silu", dropout=0.1)
+    other.load_state_dict(fused.state_dict())
+    assert other.rng_state.tolist() == [3, 4] and torch.equal(other.weight, fused.weight)
