@@ -323,7 +323,8 @@ __global__ void __launch_bounds__(1024)
 }
 
 // ----------------------------------------------------------------- backward ---
-// partial[chunk][plane] = (sum dz, sum dz xh)
+// partial[chunk][plane] = (sum dz, sum dz xh).  Slopes as exact as fp32 features': d_weight and d_bias are fp32, and the errors of
+// 16-bit features' slopes, below their rounding, would be the largest there.
 template <class T, int V, int ACT>
 __global__ void __launch_bounds__(256)
     k_gn_bwd_sums(const T *x, const T *dy, GnArgs a, const float2 *stats, const float *weight, const float *bias, float2 *partial) {
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float c = (float)v.v[j] - mean[j];
-        const float dz = j < n ? (float)d.v[j] * act_slope<ACT, T>(fmaf(c, w[j], b[j]), a.leak) : 0.f;
+        const float dz = j < n ? (float)d.v[j] * act_slope<ACT, float>(fmaf(c, w[j], b[j]), a.leak) : 0.f;
         s1[j] += dz;
         s2[j] = fmaf(dz, c * rstd[j], s2[j]);
       }

@@ -67,8 +67,9 @@ def check_group_norm(got, x, lengths, groups, weight, bias, eps, activation, lea
     bound = 1.13 * ez + (8 * U + approx) * (o["z"].abs() + 1) * (activation != "leaky_relu") + h * o["y"].abs()
     check(got[0], o["y"], bound * 1.01, what + " y")
     dz = dy.double() * o["slope"]
-    e_slope = 0.8 * ez * (activation != "leaky_relu") + (8 * U + approx) * (1 + o["z"].abs()) + U
-    e_dz = dy.double().abs() * e_slope
+    slope_error = lambda approx: 0.8 * ez * (activation != "leaky_relu") + (8 * U + approx) * (1 + o["z"].abs()) + U  # noqa: E731
+    # (the sums, which are stored in fp32, are made of fp32's slopes whatever the features are)
+    e_dx_dz, e_dz = dy.double().abs() * slope_error(approx), dy.double().abs() * slope_error(APPROX[torch.float32])
     e_xh = U * (n_stat * spread + far)
     # sums over a sample: relative to the absolute terms, plus the terms' own errors
     e_dx = torch.zeros_like(dz)
@@ -85,7 +86,7 @@ def check_group_norm(got, x, lengths, groups, weight, bias, eps, activation, lea
         e1 = mean((e_dz[rows] + n_stat * U * adz) * w)
         e2 = mean((e_dz[rows] * ax + adz * e_xh[rows] + n_stat * U * adz * ax) * w)
         terms = dz[rows].abs() * w + o["m1"][rows].abs() + (o["xh"][rows] * o["m2"][rows]).abs()
-        e_dx[rows] = o["rstd"][rows] * (e_dz[rows] * w + e1 + ax * e2 + e_xh[rows] * o["m2"][rows].abs() + n_stat * U * terms)
+        e_dx[rows] = o["rstd"][rows] * (e_dx_dz[rows] * w + e1 + ax * e2 + e_xh[rows] * o["m2"][rows].abs() + n_stat * U * terms)
     check(got[1], o["dx"], 1.01 * (e_dx + h * o["dx"].abs()), what + " dx")
     if weight is not None:
         check(got[2], o["dw"], 1.01 * (e_dw + U * o["dw"].abs()) + 1e-30, what + " dweight")
