@@ -44,6 +44,14 @@ __device__ __forceinline__ bool gn_chunk(const GnArgs &a, int64_t b, int &s, int
   return start <= r0 && r0 < r1;  // (the first: offsets that do not ascend are never followed outside of the tensor)
 }
 
+// The apply passes take the chunks from the last to the first, eight at a time: what the sums pass read last is still in the XCD's L2
+// (workgroup ids go round the 8 of them, chunk b stays on b % 8) and in the memory-side cache: 600k x 64 in fp32, a train pass, 226 us;
+// 234 from the first to the last.
+__device__ __forceinline__ int64_t gn_backwards(int chunk_blocks) {
+  const int b = blockIdx.x;
+  return (int64_t)(((chunk_blocks + 7) / 8 - 1 - b / 8) * 8 + b % 8);
+}
+
 // f(i, vector) for the thread's vectors of the span [0, span) of p: vector q, q + step, ...; the span's last vector may be partial,
 // its missing elements are zeros.
 template <int UNROLL, class T, int V, class F>
@@ -231,10 +239,10 @@ __global__ void __launch_bounds__(1024) k_gn_join(const float2 *partial, GnArgs 
 
 template <class T, int V, int ACT>
 __global__ void __launch_bounds__(256)
-    k_gn_apply(const T *x, T *y, GnArgs a, const float2 *stats, const float *weight, const float *bias) {
+    k_gn_apply(const T *x, T *y, GnArgs a, const float2 *stats, const float *weight, const float *bias, int chunk_blocks) {
   int s;
   int64_t r0, r1;
-  if (!gn_chunk(a, blockIdx.x, s, r0, r1)) return;
+  if (!gn_chunk(a, gn_backwards(chunk_blocks), s, r0, r1)) return;
   const int span = (int)(r1 - r0) * a.C;
   const T *p = x + r0 * a.C;
   T *o = y + r0 * a.C;
@@ -423,8 +431,9 @@ __global__ void __launch_bounds__(256)
     k_gn_bwd_apply(const T *x, const T *dy, T *dx, GnArgs a, const float2 *stats, const float *weight, const float *bias,
                    const float2 *sums, float *d_weight, float *d_bias, int chunk_blocks) {
   extern __shared__ float2 grp[];  // [G] (<dn>, <dn xh>)
-  if ((int)blockIdx.x >= chunk_blocks) {
-    const int c = ((int)blockIdx.x - chunk_blocks) * 256 + threadIdx.x;
+  const int padded = (chunk_blocks + 7) / 8 * 8;
+  if ((int)blockIdx.x >= padded) {
+    const int c = ((int)blockIdx.x - padded) * 256 + threadIdx.x;
     if (c >= a.C) return;
     double s1 = 0, s2 = 0;
     for (int s = 0; s < a.S; ++s) {
@@ -438,7 +447,7 @@ __global__ void __launch_bounds__(256)
   }
   int s;
   int64_t r0, r1;
-  if (!gn_chunk(a, blockIdx.x, s, r0, r1)) return;
+  if (!gn_chunk(a, gn_backwards(chunk_blocks), s, r0, r1)) return;
   const int64_t rows = min(a.offsets[s + 1], a.N) - max(a.offsets[s], (int64_t)0);
   for (int g = threadIdx.x; g < a.G; g += 256) {
     float m1 = 0.f, m2 = 0.f;
@@ -538,7 +547,7 @@ static int gn_forward(const void *x, void *y, float *stats, GnArgs a, const floa
   SCN_CHECK_LAUNCH();
   auto apply = act == SCN_ACT_SILU ? k_gn_apply<T, V, SCN_ACT_SILU>
                : act == SCN_ACT_GELU ? k_gn_apply<T, V, SCN_ACT_GELU> : k_gn_apply<T, V, SCN_ACT_LEAKY>;
-  apply<<<chunks, 256, 0, st>>>((const T *)x, (T *)y, a, (const float2 *)stats, weight, bias);
+  apply<<<(chunks + 7) / 8 * 8, 256, 0, st>>>((const T *)x, (T *)y, a, (const float2 *)stats, weight, bias, (int)chunks);
   SCN_CHECK_LAUNCH();
   return 0;
 }
@@ -556,7 +565,7 @@ static int gn_backward(const void *x, const void *dy, void *dx, const float *sta
   SCN_CHECK_LAUNCH();
   auto k2 = act == SCN_ACT_SILU ? k_gn_bwd_apply<T, V, SCN_ACT_SILU>
             : act == SCN_ACT_GELU ? k_gn_bwd_apply<T, V, SCN_ACT_GELU> : k_gn_bwd_apply<T, V, SCN_ACT_LEAKY>;
-  k2<<<chunks + (a.C + 255) / 256, 256, sizeof(float2) * a.G, st>>>((const T *)x, (const T *)dy, (T *)dx, a, (const float2 *)stats,
+  k2<<<(chunks + 7) / 8 * 8 + (a.C + 255) / 256, 256, sizeof(float2) * a.G, st>>>((const T *)x, (const T *)dy, (T *)dx, a, (const float2 *)stats,
                                                                   weight, bias, sums, d_weight, d_bias, (int)chunks);
   SCN_CHECK_LAUNCH();
   return 0;
