@@ -384,7 +384,6 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
       request(whole, v, f, g);
       multiply(v, f, wg);
     };
-    constexpr int PAIR = NT == 8 && FACTORS && sizeof(T) == 4 ? 1 : 2;  // (as many as the registers allow)
     for (int g0 = 0; g0 < a.groups; g0 += a.chunk_groups) {
       const int ng = min(a.chunk_groups, a.groups - g0), nf = min(ng, full - g0);
       const F *wg = wl + lane;
@@ -396,8 +395,7 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
       }
       if (STAY && NT < 8 && !FACTORS)
         for (; g + 4 <= nf; g += 4, wg += 4 * NT * 64) batch(std::integral_constant<int, 4>(), std::true_type(), g0 + g, wg);
-      if (PAIR == 2)
-        for (; g + 2 <= nf; g += 2, wg += 2 * NT * 64) batch(std::integral_constant<int, 2>(), std::true_type(), g0 + g, wg);
+      for (; g + 2 <= nf; g += 2, wg += 2 * NT * 64) batch(std::integral_constant<int, 2>(), std::true_type(), g0 + g, wg);
       for (; g < nf; ++g, wg += NT * 64) batch(std::integral_constant<int, 1>(), std::true_type(), g0 + g, wg);
       if (g < ng) batch(std::integral_constant<int, 1>(), std::false_type(), g0 + g, wg);
     }
@@ -701,13 +699,15 @@ static int by_type(int dtype, F &&f) {
   return f((_Float16)0);
 }
 
-// A launch that lays the weights out as [n_out, n_in] costs 2 to 4 us; every workgroup then fetches them by 16 bytes of a reduction
-// instead of by single values.  It pays for itself from some thousand sites on (177,001 x 128 to 512, bf16: 70 to 49 us without an
-// activation), and where the weights do not stay in LDS and every workgroup fetches all of them (four column tiles of 11 k-groups do).
-constexpr int64_t LIN_TRANSPOSE_ROWS = 4096;
+// The forward pass's weights come as [n_in, n_out].  Workgroups whose weights stay in LDS scatter them there themselves: 5,000 to 200,000
+// sites x 64..128 to 20..256 planes take 1.5 to 5 us less than with a launch (2.5 us) that lays them out as [n_out, n_in] first.  That
+// launch is needed where the weights do not stay and every workgroup fetches all of them (four column tiles of 11 k-groups do), and
+// for the eight column tiles that many outputs of 16-bit types are worth (200,000 x 128 to 256, bf16: 40.7 us, 47.6 without; to 128 30.2
+// and 29.4).
+constexpr int64_t LIN_WIDE = (int64_t)1 << 25;  // sites x n_out
 constexpr int LIN_FEW = 4;  // up to this many sites: k_linear_few
-static bool lin_transposes(int64_t N, int n_in, int dtype) {
-  return N > LIN_FEW && (N >= LIN_TRANSPOSE_ROWS || n_in * (dtype == SCN_F32 ? 4 : 2) > 11 * 64);
+static bool lin_transposes(int64_t N, int n_in, int n_out, int dtype) {
+  return N > LIN_FEW && (n_in * (dtype == SCN_F32 ? 4 : 2) > 11 * 64 || (dtype != SCN_F32 && N * n_out >= LIN_WIDE));
 }
 
 template <class T, int NT, int MODE, int X>
@@ -733,15 +733,17 @@ static int linear_launch(LinearArgs a, hipStream_t st) {
   SCN_CHECK_LAUNCH();
   return 0;
 }
-// wide column blocks read the rows least often; narrower ones while the chip is not full, or if they pad fewer planes
+// wide column blocks read the rows least often; narrower ones while the chip is not full, if they pad fewer planes, or for fp32, whose
+// matrix instructions are what counts (200,000 x 128 to 256: 148 us, 160 with eight column tiles)
 template <class T, int MODE, int X>
 static int linear_by_width(const LinearArgs &a, hipStream_t st) {
   const int64_t tiles = (a.N + LIN_ROWS - 1) / LIN_ROWS;
   auto blocks = [&](int nt) { return (a.M + 16 * nt - 1) / (16 * nt); };
   if (a.M <= 32 || tiles * blocks(4) < 256) return linear_launch<T, 2, MODE, X>(a, st);
-  if (a.M <= 64 || tiles * blocks(8) < 256 || blocks(4) < 2 * blocks(8) || (MODE == 0 && !a.transposed))
-    return linear_launch<T, 4, MODE, X>(a, st);
-  return linear_launch<T, 8, MODE, X>(a, st);
+  if constexpr (sizeof(T) == 2)
+    if (a.M > 64 && tiles * blocks(8) >= 256 && blocks(4) == 2 * blocks(8) && (MODE == 1 || a.transposed))
+      return linear_launch<T, 8, MODE, X>(a, st);
+  return linear_launch<T, 4, MODE, X>(a, st);
 }
 template <class T, int ACT>
 static int linear_forward(const LinearArgs &a, hipStream_t st) {
@@ -813,7 +815,7 @@ int scn_rng_take(int64_t *state, int64_t *used, void *stream) {
 }
 
 size_t scn_linear_forward_temp_bytes(int64_t N, int n_in, int n_out, int dtype) {
-  return lin_transposes(N, n_in, dtype) ? (size_t)n_in * n_out * (dtype == SCN_F32 ? 4 : 2) : 0;
+  return lin_transposes(N, n_in, n_out, dtype) ? (size_t)n_in * n_out * (dtype == SCN_F32 ? 4 : 2) : 0;
 }
 
 int scn_linear_forward(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_res,
@@ -841,7 +843,7 @@ int scn_linear_forward(const void *x, int64_t ldx, const void *weight, const voi
   a.threshold = drop_threshold(p);
   a.leak = (float)leakiness;
   a.up = (float)(1.0 / (1.0 - p));
-  const bool transpose = lin_transposes(N, n_in, dtype);
+  const bool transpose = lin_transposes(N, n_in, n_out, dtype);
   SCN_REQUIRE(!transpose || (temp && temp_bytes >= scn_linear_forward_temp_bytes(N, n_in, n_out, dtype)), "linear: workspace");
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);

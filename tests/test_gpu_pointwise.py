@@ -379,6 +379,28 @@ def test_linear_slices_and_empty(gpu):
     assert y.shape == (0, 6) and grads[0].shape == (0, 9) and (grads[1] == 0).all() and (grads[2] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_linear_many_outputs_are_those_of_few(gpu, dtype):
+    """a product's order of summation is that of its planes whatever the number of sites: large calls (other column blocks, weights laid
+    out anew) give the bits of small ones, which test_linear compares with float64.  (33.75 million outputs.)"""
+    from occuseg_amd import SCN
+    t, N, K, M, few = TYPES[dtype], 67500, 100, 500, 300
+    g = torch.Generator(device=gpu).manual_seed(6)
+    x, w, b, res, dy = (torch.randn(*shape, device=gpu, generator=g).to(t) for shape in ((N, K), (K, M), (M,), (N, M), (N, M)))
+    rng = torch.tensor([8, 9], device=gpu)
+
+    def run(rows, p):
+        y, factor, dx = x.new_empty(0), torch.empty(0, dtype=SCN.factor_dtype(x), device=gpu), x.new_empty(0)
+        SCN.FusedNetworkInNetwork_updateOutput(x[rows], y, w, b, res[rows], "gelu", 1, p, rng, factor)
+        SCN.FusedNetworkInNetwork_backward(x[rows], dx, dy[rows], w, None, None, "gelu", 1, p, factor)
+        return y, factor, dx
+
+    for p, parts in ((0.0, (slice(0, few), slice(N - few, N))), (0.4, (slice(0, few),))):
+        whole = run(slice(0, N), p)
+        for rows in parts:
+            assert all(torch.equal(a[rows], c) for a, c in zip(whole, run(rows, p))), (p, rows)
+
+
 def test_rows_do_not_mix(gpu):
     """a row of NaN or infinity reaches its own output and the weight's gradient only"""
     import occuseg_amd.sparseconvnet as scn
