@@ -167,7 +167,8 @@ __device__ __forceinline__ float activated(float z, bool keep, const LinearArgs 
   return value;
 }
 
-constexpr int LIN_ROWS = 128;  // rows of a workgroup's tile: 4 waves x 2 x 16
+// waves of a workgroup: all that the registers of a CU hold if the weights stay in LDS
+constexpr int lin_waves(int nt, bool stay) { return !stay ? 4 : nt == 8 ? 12 : 16; }
 
 constexpr int lin_piece(int nt) { return nt < 4 ? 16 * nt : 64; }  // planes of a tile that go through LDS together
 
@@ -178,7 +179,8 @@ constexpr int lin_piece(int nt) { return nt < 4 ? 16 * nt : 64; }  // planes of 
 // a 16-bit layer: addresses are a scalar base and one 32-bit offset a lane for all tiles, the bias is what the accumulators start
 // from, and the epilogue is compiled for each activation, with and without dropout and factors.
 template <class T, int NT, int MODE, int X, bool STAY>
-__global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
+__global__ void __launch_bounds__(64 * lin_waves(NT, STAY), NT == 8 || !STAY ? 3 : 4) k_linear(LinearArgs a) {
+  constexpr int WAVES = lin_waves(NT, STAY), THREADS = 64 * WAVES;
   constexpr int V = Elem<T>::V, KG = 4 * V;
   constexpr int PC = lin_piece(NT), PITCH = PC + 4, LPR = PC / V, RPI = 64 / LPR;  // planes, lanes a row, rows an instruction of a piece
   constexpr bool FACTORS = MODE == 1 && X != FACTOR_NONE;
@@ -189,6 +191,7 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
   float *bl = (float *)(wl + (size_t)NT * a.chunk_groups * 64);
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lq = lane >> 4;
   float *sw = bl + NT * 16 + wave * 16 * PITCH;
+  int *next = (int *)(bl + NT * 16 + WAVES * 16 * PITCH);  // the next tile of this workgroup
   // the column blocks of one row block run on one XCD (workgroup ids go round the 8 of them): its rows come from that L2 once
   const int per = a.row_blocks * a.col_blocks, id = blockIdx.x;
   int cb, rb;
@@ -210,29 +213,30 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
   RngKey key = {};
   if (MODE == 0 && a.threshold) key = rng_key(a.rng);
   const int full = a.K / KG;  // k-groups that lie inside the rows
-  const int tiles = (int)(STAY ? (a.N + 31) / 32 : (a.N + LIN_ROWS - 1) / LIN_ROWS * 4);
+  const int tiles = (int)(STAY ? (a.N + 31) / 32 : (a.N + 127) / 128 * 4);
+  if (threadIdx.x == 0) *next = WAVES;
 
   // weights of k-groups g0 .. g0 + ng in the order of the A operands, several loads a thread in flight
   auto stage = [&](int g0, int ng) __attribute__((always_inline)) {
     constexpr int B = 4;
     if (MODE == 1 || NT == 8 || !STAY || a.transposed) {  // [M, K]: a lane's V elements lie together
-      for (int e0 = threadIdx.x; e0 < NT * ng * 64; e0 += 256 * B) {
+      for (int e0 = threadIdx.x; e0 < NT * ng * 64; e0 += THREADS * B) {
         Pack<T, V> v[B];
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-          const int e = e0 + 256 * i, l = e & 63, t = (e >> 6) % NT, g = (e >> 6) / NT;
+          const int e = e0 + THREADS * i, l = e & 63, t = (e >> 6) % NT, g = (e >> 6) / NT;
           const int m = m0 + 16 * t + (l & 15), k = (g0 + g) * KG + (l >> 4) * V;
           v[i] = load_some<T, V>(wt + (int64_t)m * a.K + k, e < NT * ng * 64 && m < a.M ? a.K - k : 0);
         }
 #pragma unroll
         for (int i = 0; i < B; ++i)
-          if (e0 + 256 * i < NT * ng * 64) __builtin_memcpy(&wl[e0 + 256 * i], &v[i], 16);
+          if (e0 + THREADS * i < NT * ng * 64) __builtin_memcpy(&wl[e0 + THREADS * i], &v[i], 16);
       }
     } else {  // [K, M]: V planes of one k, spread over V lanes' places
       constexpr int MV = NT * 16 / V;  // vectors a row
       const int n = MV * ng * KG;
       T *lds = (T *)wl;
-      for (int e = threadIdx.x; e < n; e += 256) {
+      for (int e = threadIdx.x; e < n; e += THREADS) {
         const int m = e % MV * V, k = e / MV;
         const Pack<T, V> v = load_some<T, V>(wt + (int64_t)(g0 * KG + k) * a.M + m0 + m, g0 * KG + k < a.K ? a.M - m0 - m : 0);
 #pragma unroll
@@ -315,7 +319,9 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
       a.factor ? finish(whole, std::false_type(), std::true_type(), row0, pc) : finish(whole, std::false_type(), std::false_type(), row0, pc);
   };
 
-  for (int tile = rb * 4 + wave; tile < tiles; tile += a.row_blocks * 4) {
+  for (int i = wave;;) {
+    const int tile = STAY ? i * a.row_blocks + rb : rb * 4 + i;
+    if (tile >= tiles) break;
     const int64_t row0 = (int64_t)tile * 32;
     // (rows behind the last are read as the last and not written; of tiles behind the last, too)
     const int64_t base = min(row0, a.N - 1);
@@ -420,6 +426,9 @@ __global__ void __launch_bounds__(256, NT == 8 ? 3 : 4) k_linear(LinearArgs a) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
+    if constexpr (!STAY) break;
+    if (lane == 0) i = atomicAdd(next, 1);
+    i = __builtin_amdgcn_readfirstlane(i);
   }
 }
 
@@ -705,31 +714,36 @@ static int by_type(int dtype, F &&f) {
 // for the eight column tiles that many outputs of 16-bit types are worth (200,000 x 128 to 256, bf16: 40.7 us, 47.6 without; to 128 30.2
 // and 29.4).
 constexpr int64_t LIN_WIDE = (int64_t)1 << 25;  // sites x n_out
+constexpr int LIN_LDS = 163840;
 constexpr int LIN_FEW = 4;  // up to this many sites: k_linear_few
 static bool lin_transposes(int64_t N, int n_in, int n_out, int dtype) {
-  return N > LIN_FEW && (n_in * (dtype == SCN_F32 ? 4 : 2) > 11 * 64 || (dtype != SCN_F32 && N * n_out >= LIN_WIDE));
+  return N > LIN_FEW && (n_in * (dtype == SCN_F32 ? 4 : 2) > 22 * 64 || (dtype != SCN_F32 && N * n_out >= LIN_WIDE));
 }
 
 template <class T, int NT, int MODE, int X>
 static int linear_launch(LinearArgs a, hipStream_t st) {
   constexpr int KG = 4 * Elem<T>::V, group_bytes = NT * 64 * 16;
+  auto rest = [](int waves) { return NT * 16 * 4 + waves * 16 * (lin_piece(NT) + 4) * 4 + 16; };  // bias, results, next tile
   a.groups = (a.K + KG - 1) / KG;
   a.chunk_groups = a.groups;
-  const size_t rest = NT * 16 * 4 + 4 * 16 * (lin_piece(NT) + 4) * 4;  // bias, results
-  if (a.groups * group_bytes + rest > 65536) a.chunk_groups = 32768 / group_bytes;
   a.col_blocks = (a.M + NT * 16 - 1) / (NT * 16);
-  const int64_t tiles = (a.N + LIN_ROWS - 1) / LIN_ROWS;
-  const size_t lds = (size_t)a.chunk_groups * group_bytes + rest;
-  // as many workgroups as the CUs hold, a multiple of the XCDs; weights that do not stay: one tile a workgroup
-  int64_t fit = 163840 / (int64_t)lds;
-  if (fit > (NT == 8 ? 3 : 4)) fit = NT == 8 ? 3 : 4;
-  int64_t rows = 256 * fit / a.col_blocks / 8 * 8;
-  if (rows < 8) rows = 8;
-  if (a.groups > a.chunk_groups || rows > tiles) rows = tiles;
-  SCN_REQUIRE(rows * a.col_blocks < ((int64_t)1 << 24), "linear: sites x planes beyond a launch of 2^32 threads");
+  const bool stay = a.groups * group_bytes + rest(lin_waves(NT, true)) <= LIN_LDS;
+  int64_t rows, lds;
+  if (stay) {  // one workgroup a CU, the column blocks of a row block on one XCD
+    rows = a.col_blocks <= 32 ? 32 / a.col_blocks * 8 : 256 / a.col_blocks;
+    const int64_t tiles = (a.N + 31) / 32;
+    if (rows > tiles) rows = tiles;
+    if (rows < 1) rows = 1;
+    lds = a.groups * group_bytes + rest(lin_waves(NT, true));
+  } else {
+    a.chunk_groups = 32768 / group_bytes;
+    rows = (a.N + 127) / 128;
+    lds = a.chunk_groups * group_bytes + rest(lin_waves(NT, false));
+  }
+  SCN_REQUIRE(rows * a.col_blocks < ((int64_t)1 << 22), "linear: sites x planes beyond a launch of 2^32 threads");
   a.row_blocks = (int)rows;
-  auto k = a.groups <= a.chunk_groups ? k_linear<T, NT, MODE, X, true> : k_linear<T, NT, MODE, X, false>;
-  k<<<(unsigned)(rows * a.col_blocks), 256, lds, st>>>(a);
+  auto k = stay ? k_linear<T, NT, MODE, X, true> : k_linear<T, NT, MODE, X, false>;
+  k<<<(unsigned)(rows * a.col_blocks), 64 * lin_waves(NT, stay), lds, st>>>(a);
   SCN_CHECK_LAUNCH();
   return 0;
 }
@@ -737,7 +751,7 @@ static int linear_launch(LinearArgs a, hipStream_t st) {
 // matrix instructions are what counts (200,000 x 128 to 256: 148 us, 160 with eight column tiles)
 template <class T, int MODE, int X>
 static int linear_by_width(const LinearArgs &a, hipStream_t st) {
-  const int64_t tiles = (a.N + LIN_ROWS - 1) / LIN_ROWS;
+  const int64_t tiles = (a.N + 127) / 128;
   auto blocks = [&](int nt) { return (a.M + 16 * nt - 1) / (16 * nt); };
   if (a.M <= 32 || tiles * blocks(4) < 256) return linear_launch<T, 2, MODE, X>(a, st);
   if constexpr (sizeof(T) == 2)
