@@ -469,7 +469,8 @@ int scn_sample_offsets(const uint64_t *site_keys, int64_t N, int64_t samples, in
 /* y = act((x - mean) rstd weight + bias), mean and 1 / rstd^2 - eps the mean and variance of the sites of one sample and the
  * planes / groups planes of one group.  offsets int64 [samples + 1] ascending in 0..N; rows in front of the first sample and
  * behind the last are neither read nor written.  weight / bias fp32 [planes] or NULL; stats fp32 [samples][groups][2] = (mean,
- * rstd), zeros for a sample without sites.  x and y contiguous; temp: scn_group_norm_temp_bytes. */
+ * rstd), zeros for a sample without sites.  x and y contiguous; temp: scn_group_norm_temp_bytes (0: may
+ * be NULL). */
 size_t scn_group_norm_temp_bytes(int64_t N, int planes, int groups, int64_t samples, int dtype, int backward);
 int scn_group_norm_forward(const void *x, void *y, float *stats, const int64_t *offsets, const float *weight,
                            const float *bias, double eps, int act, double leakiness, int64_t N, int planes, int groups,

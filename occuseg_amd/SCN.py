@@ -1985,7 +1985,7 @@ def GroupNormalization_updateOutput(input_features, output_features, stats, offs
         _sized(output_features, x.dtype, device, N, C)
         _sized(stats, torch.float32, device, S, groups, 2)
         tb = lib.scn_group_norm_temp_bytes(N, C, groups, S, code, 0)
-        temp = torch.empty(tb, dtype=torch.uint8, device=x.device)
+        temp = torch.empty(tb, dtype=torch.uint8, device=x.device) if tb else None
         ev = _prof_begin("bn")
         check(lib.scn_group_norm_forward(ptr(x), ptr(output_features), ptr(stats), ptr(offsets), ptr(weight), ptr(bias),
                                          float(eps), act, float(leakiness), N, C, groups, S, code, ptr(temp), tb, stream()))

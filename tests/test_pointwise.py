@@ -75,9 +75,10 @@ def test_boundary_refuses_on_the_host():
     with pytest.raises(RuntimeError, match="GPU"):
         SCN.GroupNormalization_updateOutput(torch.zeros(2, 4), e, e, torch.zeros(2, dtype=torch.int64), None, None, 1e-4, 2, "silu", 1)
     # the C entries look at their arguments before they launch anything
-    assert lib.scn_group_norm_temp_bytes(100, 8, 3, 1, 0, 0) == 0 and lib.scn_group_norm_temp_bytes(100, 8, 2, 1, 0, 0) > 0
+    assert lib.scn_group_norm_temp_bytes(100, 8, 3, 1, 0, 0) == 0 and lib.scn_group_norm_temp_bytes(100, 8, 2, 1, 0, 1) > 0
     assert lib.scn_group_norm_forward(None, None, None, None, None, None, 1e-4, 0, 1.0, 10, 8, 2, 1, 0, None, 0, None) == 2
     assert lib.scn_group_norm_forward(None, None, None, None, None, None, 1e-4, 7, 1.0, 10, 8, 2, 1, 0, None, 0, None) == 2
+    assert lib.scn_group_norm_temp_bytes(100, 8, 2, 1, 0, 0) == 0 and lib.scn_group_norm_temp_bytes(10000, 8, 2, 1, 0, 0) > 0
     assert lib.scn_group_norm_backward(None, None, None, None, None, None, None, None, None, 0, 1.0, 10, 8, 2, 1, 3, None, 0, None) == 2
     assert lib.scn_dropout(None, 8, None, 10, 8, 0, 0.5, None, None) == 2
     assert lib.scn_dropout(None, 8, None, 10, 8, 0, 1.0, None, None) == 2
