@@ -4,13 +4,13 @@
 //              dx = dz W^T;  dW = x^T dz;  db = column sums of dz
 //
 // Sites are many (up to 600k) and planes few (16 to 512), so the products are HBM bound but for the widest: 2 n_in n_out flops for
-// n_in + n_out values, 16 to 128 flops a byte where fp32 MFMA balances at 20 and bf16 at 300.  Everything that belongs to a row is
+// n_in + n_out values, 16 to 128 flops a byte where fp32 MFMA balances at 28 and bf16 at 200.  Everything that belongs to a row is
 // done while it is in registers.
 //
 // Products: v_mfma 16x16, the WEIGHT as the A operand and the sites as B: the four results of a lane are then four consecutive
-// planes of one site.  The order of the
-// reduction is free as long as both operands agree: a lane's 16 bytes of a row, loaded straight from global memory, ARE its B
-// operands (one 16x16x32 of 16-bit types, four 16x16x4 of fp32).  The weights are laid out in LDS in the order of the A operands.
+// planes of one site.  The order of the reduction is free as long as both operands agree: a lane's 16 bytes of a row, loaded straight
+// from global memory, ARE its B operands (one 16x16x32 of 16-bit types, four 16x16x4 of fp32).  The weights are laid out in LDS in the
+// order of the A operands.
 #include "scn_pointwise.h"
 
 namespace scn {
@@ -47,7 +47,8 @@ __device__ __forceinline__ void store_some(T *p, const Pack<T, V> &v, int n) {
 
 // ------------------------------------------------------------------- dropout ---
 // Every element read and written once; the mask is made of the counter.  A thread keeps its planes -- Q quads -- and walks the
-// sites, `rows` of a step at a time: the products of the counter that belong to the planes are made once.
+// sites, `rows` of a step at a time: the products of the counter that belong to the planes are made once.  Four rows are requested
+// before the first is used.  HBM bound: 601,674 x 128 bf16 take 62 us = 5.0 TB/s, a copy of as many bytes 57.
 template <class T, int Q, bool WHOLE>
 __global__ void __launch_bounds__(256)
     k_dropout(const T *x, int64_t ldx, T *y, int64_t N, int C, int items, int rows, uint32_t threshold, float scale, const int64_t *rng) {
@@ -173,11 +174,16 @@ constexpr int lin_waves(int nt, bool stay) { return !stay ? 4 : nt == 8 ? 12 : 1
 constexpr int lin_piece(int nt) { return nt < 4 ? 16 * nt : 64; }  // planes of a tile that go through LDS together
 
 // MODE 0: forward with the epilogue, X its activation.  MODE 1: dx, X how the factors are stored.
-// A workgroup holds the weights of NT x 16 output planes in LDS -- all of K, once, if they fit (STAY): then its waves walk 32-row tiles
-// of their own without a barrier -- else `chunk_groups` at a time, and its waves keep together.
+// A workgroup holds the weights of NT x 16 output planes in LDS -- all of K, once, if they fit (STAY): then it has a CU to itself and
+// its waves take 32-row tiles without a barrier -- else `chunk_groups` at a time, and its waves keep together.  Tiles are taken from a
+// counter in LDS: the older of the waves on a SIMD come first at its matrix pipe and take 15 us a tile where the youngest take 37
+// (200,000 x 128 to 128, fp32), so that equal shares end at 50 to 85 us.
 // Beside fp32 MFMAs a vector instruction costs 8 or more of the matrix pipe's cycles, and the epilogue alone fills half the time of
 // a 16-bit layer: addresses are a scalar base and one 32-bit offset a lane for all tiles, the bias is what the accumulators start
 // from, and the epilogue is compiled for each activation, with and without dropout and factors.
+// Measured: 601,674 x 64 to 20, fp32, 40 us = 5.1 TB/s; 177,001 x 64 to 128, fp32, GELU, dropout, residual and factors, 66 us = 4.8 TB/s
+// (forward), 42 us = 5.4 TB/s (dx); 177,001 x 128 to 512, bf16, GELU, dropout and factors, 126 us = 3.2 TB/s (forward: some 37 vector
+// instructions an output), 102 us = 4.0 TB/s (dx); fp32 that is not bound by memory: 200,000 x 128 to 128 80 us = 82 TFLOP/s.
 template <class T, int NT, int MODE, int X, bool STAY>
 __global__ void __launch_bounds__(64 * lin_waves(NT, STAY), NT == 8 || !STAY ? 3 : 4) k_linear(LinearArgs a) {
   constexpr int WAVES = lin_waves(NT, STAY), THREADS = 64 * WAVES;
@@ -509,6 +515,8 @@ __global__ void __launch_bounds__(1024) k_linear_few(LinearArgs a) {
 // loaded element by element (the last rows of the last slice).
 // Workgroup (slice, tile): four waves take the slice's row steps in turn, join through LDS and write one slab; slabs are added by
 // k_linear_dw_join in slice order.
+// HBM bound, with the join: 177,001 x 64 to 128, fp32, with factors 52 us = 4.3 TB/s; 128 to 512, bf16, 104 us = 3.9 TB/s (without
+// factors 53 us = 4.3 TB/s).  Few sites: a step's latency three times over, the waves' join and the slabs, 18 us for 50,001 x 35 to 77.
 struct DwArgs {
   const void *x, *dy, *factor;
   int64_t ldx, ld_dy, N;

@@ -401,6 +401,26 @@ def test_linear_many_outputs_are_those_of_few(gpu, dtype):
             assert all(torch.equal(a[rows], c) for a, c in zip(whole, run(rows, p))), (p, rows)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("K,M", [(352, 64), (353, 64), (704, 64), (705, 64), (128, 416), (128, 417), (64, 353), (64, 705)])
+def test_linear_weights_that_just_fit(gpu, K, M, dtype):
+    """both sides of where the weights of a column block stop staying on a CU: the bits of small calls, as above"""
+    from occuseg_amd import SCN
+    t, N, few = TYPES[dtype], 33000, 200
+    g = torch.Generator(device=gpu).manual_seed(7)
+    x, w, b, dy = (torch.randn(*shape, device=gpu, generator=g).to(t) for shape in ((N, K), (K, M), (M,), (N, M)))
+
+    def run(rows):
+        y, factor, dx = x.new_empty(0), torch.empty(0, dtype=SCN.factor_dtype(x), device=gpu), x.new_empty(0)
+        SCN.FusedNetworkInNetwork_updateOutput(x[rows], y, w, b, None, "silu", 1, 0.0, None, factor)
+        SCN.FusedNetworkInNetwork_backward(x[rows], dx, dy[rows], w, None, None, "silu", 1, 0.0, factor)
+        return y, factor, dx
+
+    whole = run(slice(0, N))
+    for rows in (slice(0, few), slice(N - few, N)):
+        assert all(torch.equal(a[rows], c) for a, c in zip(whole, run(rows))), rows
+
+
 def test_rows_do_not_mix(gpu):
     """a row of NaN or infinity reaches its own output and the weight's gradient only"""
     import occuseg_amd.sparseconvnet as scn
