@@ -172,6 +172,10 @@ __device__ __forceinline__ float activated(float z, bool keep, const LinearArgs 
 constexpr int lin_waves(int nt, bool stay) { return !stay ? 4 : nt == 8 ? 12 : 16; }
 
 constexpr int lin_piece(int nt) { return nt < 4 ? 16 * nt : 64; }  // planes of a tile that go through LDS together
+// ... as the sums they are, or, where nothing but a factor is missing, as the 16-bit values that will be stored: half the room, so the
+// weights of 512 planes stay (dx of 177,001 x 128 to 512, bf16: 103 to 92 us)
+constexpr bool lin_packed(int mode, int size) { return mode == 1 && size == 2; }
+constexpr int lin_piece_bytes(int nt, bool packed) { return packed ? 16 * (lin_piece(nt) + 8) * 2 : 16 * (lin_piece(nt) + 4) * 4; }
 
 // MODE 0: forward with the epilogue, X its activation.  MODE 1: dx, X how the factors are stored.
 // A workgroup holds the weights of NT x 16 output planes in LDS -- all of K, once, if they fit (STAY): then it has a CU to itself and
@@ -183,12 +187,13 @@ constexpr int lin_piece(int nt) { return nt < 4 ? 16 * nt : 64; }  // planes of 
 // from, and the epilogue is compiled for each activation, with and without dropout and factors.
 // Measured: 601,674 x 64 to 20, fp32, 40 us = 5.1 TB/s; 177,001 x 64 to 128, fp32, GELU, dropout, residual and factors, 66 us = 4.8 TB/s
 // (forward), 42 us = 5.4 TB/s (dx); 177,001 x 128 to 512, bf16, GELU, dropout and factors, 126 us = 3.2 TB/s (forward: some 37 vector
-// instructions an output), 102 us = 4.0 TB/s (dx); fp32 that is not bound by memory: 200,000 x 128 to 128 80 us = 82 TFLOP/s.
+// instructions an output), 92 us = 4.4 TB/s (dx; a plain sum reads 4.0 to 4.9); fp32 that is not bound by memory: 200,000 x 128 to 128 80 us = 82 TFLOP/s.
 template <class T, int NT, int MODE, int X, bool STAY>
 __global__ void __launch_bounds__(64 * lin_waves(NT, STAY), NT == 8 || !STAY ? 3 : 4) k_linear(LinearArgs a) {
   constexpr int WAVES = lin_waves(NT, STAY), THREADS = 64 * WAVES;
   constexpr int V = Elem<T>::V, KG = 4 * V;
-  constexpr int PC = lin_piece(NT), PITCH = PC + 4, LPR = PC / V, RPI = 64 / LPR;  // planes, lanes a row, rows an instruction of a piece
+  constexpr bool PACKED = lin_packed(MODE, sizeof(T));
+  constexpr int PC = lin_piece(NT), PITCH = PACKED ? PC + 8 : PC + 4, LPR = PC / V, RPI = 64 / LPR;  // planes, lanes a row, rows an instruction of a piece
   constexpr bool FACTORS = MODE == 1 && X != FACTOR_NONE;
   using F = typename Frag<T>::type;
   using Q = typename FactorOf<T>::type;
@@ -196,8 +201,8 @@ __global__ void __launch_bounds__(64 * lin_waves(NT, STAY), NT == 8 || !STAY ? 3
   F *wl = (F *)smem;  // [k-group of the chunk][tile][lane]
   float *bl = (float *)(wl + (size_t)NT * a.chunk_groups * 64);
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lq = lane >> 4;
-  float *sw = bl + NT * 16 + wave * 16 * PITCH;
-  int *next = (int *)(bl + NT * 16 + WAVES * 16 * PITCH);  // the next tile of this workgroup
+  float *sw = bl + NT * 16 + wave * (lin_piece_bytes(NT, PACKED) / 4);
+  int *next = (int *)(bl + NT * 16 + WAVES * (lin_piece_bytes(NT, PACKED) / 4));  // the next tile of this workgroup
   // the column blocks of one row block run on one XCD (workgroup ids go round the 8 of them): its rows come from that L2 once
   const int per = a.row_blocks * a.col_blocks, id = blockIdx.x;
   int cb, rb;
@@ -273,6 +278,16 @@ __global__ void __launch_bounds__(64 * lin_waves(NT, STAY), NT == 8 || !STAY ? 3
         const T *p = res + (int64_t)(i * RPI) * a.ld_res + res0;
         rv[i] = WHOLE ? load_pack<T, V>(p) : load_some<T, V>(p, i * RPI + r0 < rows ? left : 0);
       }
+    if constexpr (PACKED) {
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const Pack<T, V> y = load_pack<T, V>((const T *)sw + (i * RPI + r0) * PITCH + c);
+        T *o = out + (int64_t)(i * RPI) * a.M + o0;
+        if constexpr (WHOLE) store_pack<T, V>(o, y);
+        else if (i * RPI + r0 < rows) store_some<T, V>(o, y, left);
+      }
+      return;
+    }
     float z[IT][V];
 #pragma unroll
     for (int i = 0; i < IT; ++i)
@@ -421,7 +436,12 @@ __global__ void __launch_bounds__(64 * lin_waves(NT, STAY), NT == 8 || !STAY ? 3
       for (int k = 0; k < 2 * PPU; ++k)
         if (k == piece) {
 #pragma unroll
-          for (int t = 0; t < PC / 16; ++t) *(floatx4 *)(sw + li * PITCH + 16 * t + 4 * lq) = acc[k / PPU][k % PPU * (PC / 16) + t];
+          for (int t = 0; t < PC / 16; ++t) {
+            const floatx4 v = acc[k / PPU][k % PPU * (PC / 16) + t];
+            if constexpr (PACKED)
+              store_pack<T, 4>((T *)sw + li * PITCH + 16 * t + 4 * lq, {{(T)(v[0] * a.up), (T)(v[1] * a.up), (T)(v[2] * a.up), (T)(v[3] * a.up)}});
+            else *(floatx4 *)(sw + li * PITCH + 16 * t + 4 * lq) = v;
+          }
         }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -731,7 +751,8 @@ static bool lin_transposes(int64_t N, int n_in, int n_out, int dtype) {
 template <class T, int NT, int MODE, int X>
 static int linear_launch(LinearArgs a, hipStream_t st) {
   constexpr int KG = 4 * Elem<T>::V, group_bytes = NT * 64 * 16;
-  auto rest = [](int waves) { return NT * 16 * 4 + waves * 16 * (lin_piece(NT) + 4) * 4 + 16; };  // bias, results, next tile
+  // bias, results, next tile
+  auto rest = [](int waves) { return NT * 16 * 4 + waves * lin_piece_bytes(NT, lin_packed(MODE, sizeof(T))) + 16; };
   a.groups = (a.K + KG - 1) / KG;
   a.chunk_groups = a.groups;
   a.col_blocks = (a.M + NT * 16 - 1) / (NT * 16);
