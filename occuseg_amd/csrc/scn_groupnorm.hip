@@ -114,13 +114,28 @@ __device__ __forceinline__ void gn_store(T *p, int n, const Pack<T, V> &v) {
       if (j < n) p[j] = v.v[j];
 }
 
-// f(j, plane, group) for the V planes of vector q
+// f(j, plane's group, (mean, rstd), weight, bias) for the V planes of vector q in sample s.  Planes that lie side by side come by 16
+// bytes, and one pair of statistics serves them all if they are of one group: 8 planes take 5 loads instead of 24.
 template <int V, class F>
-__device__ __forceinline__ void gn_planes(const GnArgs &a, int q, F &&f) {
+__device__ __forceinline__ void gn_planes(const GnArgs &a, int q, const float2 *stats, const float *weight, const float *bias, F &&f) {
   int c = q * V % a.C, g = c / a.cpg, r = c % a.cpg;
+  if (a.C % V == 0) {
+    Pack<float, V> w, b;
+#pragma unroll
+    for (int j = 0; j < V; ++j) w.v[j] = 1.f, b.v[j] = 0.f;
+    if (weight) w = load_pack<float, V>(weight + c);
+    if (bias) b = load_pack<float, V>(bias + c);
+    float2 st = stats[g];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      f(j, g, st, w.v[j], b.v[j]);
+      if (j < V - 1 && ++r == a.cpg) r = 0, st = stats[++g];
+    }
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    f(j, c, g);
+    f(j, g, stats[g], weight ? weight[c] : 1.f, bias ? bias[c] : 0.f);
     ++c;
     if (++r == a.cpg) r = 0, ++g;
     if (c == a.C) c = g = 0;
@@ -248,11 +263,10 @@ __global__ void __launch_bounds__(256)
   T *o = y + r0 * a.C;
   for (int q = threadIdx.x; q < a.step; q += 256) {
     float mean[V], w[V], b[V];
-    gn_planes<V>(a, q, [&](int j, int c, int gi) {
-      const float2 st = stats[(int64_t)s * a.G + gi];
+    gn_planes<V>(a, q, stats + (int64_t)s * a.G, weight, bias, [&](int j, int, float2 st, float wj, float bj) {
       mean[j] = st.x;
-      w[j] = st.y * (weight ? weight[c] : 1.f);
-      b[j] = bias ? bias[c] : 0.f;
+      w[j] = st.y * wj;
+      b[j] = bj;
     });
     gn_walk<4, T, V>(p, span, q, a.step, [&](int i, int n, const Pack<T, V> &v) {
       Pack<T, V> r;
@@ -345,12 +359,11 @@ __global__ void __launch_bounds__(256)
   const T *p = x + r0 * a.C, *g = dy + r0 * a.C;
   for (int q = threadIdx.x; q < a.step; q += 256) {
     float mean[V], rstd[V], w[V], b[V], s1[V], s2[V];
-    gn_planes<V>(a, q, [&](int j, int c, int gi) {
-      const float2 st = stats[(int64_t)s * a.G + gi];
+    gn_planes<V>(a, q, stats + (int64_t)s * a.G, weight, bias, [&](int j, int, float2 st, float wj, float bj) {
       mean[j] = st.x;
       rstd[j] = st.y;
-      w[j] = st.y * (weight ? weight[c] : 1.f);
-      b[j] = bias ? bias[c] : 0.f;
+      w[j] = st.y * wj;
+      b[j] = bj;
       s1[j] = s2[j] = 0.f;
     });
     gn_walk2<4, T, V>(p, g, span, q, a.step, [&](int i, int n, const Pack<T, V> &v, const Pack<T, V> &d) {
@@ -467,11 +480,10 @@ __global__ void __launch_bounds__(256)
   T *o = dx + r0 * a.C;
   for (int q = threadIdx.x; q < a.step; q += 256) {
     float mean[V], w[V], b[V], m1[V], m2[V];
-    gn_planes<V>(a, q, [&](int j, int c, int gi) {
-      const float2 st = stats[(int64_t)s * a.G + gi];
+    gn_planes<V>(a, q, stats + (int64_t)s * a.G, weight, bias, [&](int j, int gi, float2 st, float wj, float bj) {
       mean[j] = st.x;
-      w[j] = st.y * (weight ? weight[c] : 1.f);
-      b[j] = bias ? bias[c] : 0.f;
+      w[j] = st.y * wj;
+      b[j] = bj;
       m1[j] = grp[gi].x * st.y;
       m2[j] = grp[gi].y * st.y * st.y;
     });
