@@ -530,9 +530,9 @@ static GnArgs gn_args(const int64_t *offsets, int64_t N, int C, int G, int64_t S
   a.leak = (float)leak;
   a.period = C / gcd(C, V);
   a.step = a.period <= 256 ? 256 / a.period * a.period : a.period;
-  // Chunks of 32 KB (fp32) or 64 KB (16 bits; a thread's constants are twice as many) of a large tensor: 154 MB in fp32 take 97 us
-  // forwards with 32 KB, 103 with 64; 45 MB in bf16 36 with 64 KB, 40 with 32, 54 with 16.  Of a small one 512 chunks, none below 16 KB.
-  const int64_t row = (int64_t)C * (dtype == SCN_F32 ? 4 : 2), most = dtype == SCN_F32 ? 32768 : 65536;
+  // Chunks of 32 KB of a large tensor: 154 MB in fp32 take 91 us forwards, 100 with 16 KB; 45 MB in bf16 36, 38 with 64 KB.  Of a small one
+  // 512 chunks, none below 16 KB.
+  const int64_t row = (int64_t)C * (dtype == SCN_F32 ? 4 : 2), most = 32768;
   int64_t bytes = N * row / 512;
   bytes = bytes < 16384 ? 16384 : bytes > most ? most : bytes;
   a.shift = 0;
