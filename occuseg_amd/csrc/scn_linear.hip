@@ -186,7 +186,7 @@ constexpr int lin_piece_bytes(int nt, bool packed) { return packed ? 16 * (lin_p
 // a 16-bit layer: addresses are a scalar base and one 32-bit offset a lane for all tiles, the bias is what the accumulators start
 // from, and the epilogue is compiled for each activation, with and without dropout and factors.
 // Measured: 601,674 x 64 to 20, fp32, 40 us = 5.1 TB/s; 177,001 x 64 to 128, fp32, GELU, dropout, residual and factors, 66 us = 4.8 TB/s
-// (forward), 42 us = 5.4 TB/s (dx); 177,001 x 128 to 512, bf16, GELU, dropout and factors, 126 us = 3.2 TB/s (forward: some 37 vector
+// (forward), 42 us = 5.4 TB/s (dx); 177,001 x 128 to 512, bf16, GELU, dropout and factors, 118 us = 3.4 TB/s (forward: some 37 vector
 // instructions an output), 92 us = 4.4 TB/s (dx; a plain sum reads 4.0 to 4.9); fp32 that is not bound by memory: 200,000 x 128 to 128 80 us = 82 TFLOP/s.
 template <class T, int NT, int MODE, int X, bool STAY>
 __global__ void __launch_bounds__(64 * lin_waves(NT, STAY), NT == 8 || !STAY ? 3 : 4) k_linear(LinearArgs a) {
@@ -738,14 +738,19 @@ static int by_type(int dtype, F &&f) {
 
 // The forward pass's weights come as [n_in, n_out].  Workgroups whose weights stay in LDS scatter them there themselves: 5,000 to 200,000
 // sites x 64..128 to 20..256 planes take 1.5 to 5 us less than with a launch (2.5 us) that lays them out as [n_out, n_in] first.  That
-// launch is needed where the weights do not stay and every workgroup fetches all of them (four column tiles of 11 k-groups do), and
+// launch is needed where the weights do not stay and every workgroup fetches all of them (four column tiles of 22 k-groups do), and
 // for the eight column tiles that many outputs of 16-bit types are worth (200,000 x 128 to 256, bf16: 40.7 us, 47.6 without; to 128 30.2
-// and 29.4).
+// and 29.4; 600,000 x 448 to 256, where eight do not stay and four do, 308 and 338).
 constexpr int64_t LIN_WIDE = (int64_t)1 << 25;  // sites x n_out
-constexpr int LIN_LDS = 163840;
+constexpr int LIN_LDS = 163840;  // of a CU
 constexpr int LIN_FEW = 4;  // up to this many sites: k_linear_few
+// eight column tiles fill the chip and pad no more than four
+static bool lin_wide(int64_t N, int M) {
+  return M > 64 && (N + 127) / 128 * ((M + 127) / 128) >= 256 && (M + 63) / 64 == 2 * ((M + 127) / 128);
+}
 static bool lin_transposes(int64_t N, int n_in, int n_out, int dtype) {
-  return N > LIN_FEW && (n_in * (dtype == SCN_F32 ? 4 : 2) > 22 * 64 || (dtype != SCN_F32 && N * n_out >= LIN_WIDE));
+  const int row = n_in * (dtype == SCN_F32 ? 4 : 2);
+  return N > LIN_FEW && (row > 22 * 64 || (dtype != SCN_F32 && N * n_out >= LIN_WIDE && lin_wide(N, n_out)));
 }
 
 template <class T, int NT, int MODE, int X>
@@ -780,12 +785,9 @@ static int linear_launch(LinearArgs a, hipStream_t st) {
 // matrix instructions are what counts (200,000 x 128 to 256: 148 us, 160 with eight column tiles)
 template <class T, int MODE, int X>
 static int linear_by_width(const LinearArgs &a, hipStream_t st) {
-  const int64_t tiles = (a.N + 127) / 128;
-  auto blocks = [&](int nt) { return (a.M + 16 * nt - 1) / (16 * nt); };
-  if (a.M <= 32 || tiles * blocks(4) < 256) return linear_launch<T, 2, MODE, X>(a, st);
+  if (a.M <= 32 || (a.N + 127) / 128 * ((a.M + 63) / 64) < 256) return linear_launch<T, 2, MODE, X>(a, st);
   if constexpr (sizeof(T) == 2)
-    if (a.M > 64 && tiles * blocks(8) >= 256 && blocks(4) == 2 * blocks(8) && (MODE == 1 || a.transposed))
-      return linear_launch<T, 8, MODE, X>(a, st);
+    if (lin_wide(a.N, a.M) && (MODE == 1 || a.transposed)) return linear_launch<T, 8, MODE, X>(a, st);
   return linear_launch<T, 4, MODE, X>(a, st);
 }
 template <class T, int ACT>
