@@ -8,7 +8,6 @@
 #   5. PMC groups on the isolated gather-mm layers (tools/pmc_groups.sh)      -> pmc_conv_tile4.txt
 #   6. MFMA issue probe, occupancy probe, kernel A/Bs                          -> mfma_probe.txt, occupancy_probe.txt, ab_*.txt
 #   7. memory-safety runs of the train step (tools/guard_run.py: guard pages at either end of every tensor)  -> guard_*.txt
-#   8. the sort's scratch under the profiler (tools/scratch_fault_repro.sh)      -> scratch_fault_repro.txt
 # --pmc runs use --kernel-trace only (the pool refuses PMC together with the hip/hsa trace domains).  Every rocprofv3 run is
 # under `timeout`: after a GPU fault the profiler does not exit by itself (round 3, evidence run 3: 40 minutes).
 set -u
