@@ -120,18 +120,29 @@ __device__ __forceinline__ floatx4 mma(const halfx8 &a, const halfx8 &b, const f
 // slopes rounded to the same type would make that rounding twice, so they are kept finer:
 //   FACTOR_FLOAT  fp32 features: fp32
 //   FACTOR_HALF   bf16 features: fp16, 2^-12 of a slope
-//   FACTOR_FIXED  fp16 features: 16 bits of fixed point, 2^-15 (the smooth activations' slopes are below 1.13); -2^15: NaN
+//   FACTOR_SHORT  fp16 features: sign, 4 bits of exponent, 11 of mantissa: 2^-12 of a slope from 2^-14 to 2 (the smooth activations'
+//                 are below 1.13), 2^-26 below, where dz itself is among fp16's subnormal numbers; 0x7fff: NaN
 //   FACTOR_SIGN   leaky ReLU of 16-bit features, whose slope may be any number: 2: 1, 1: leak, 0: dropped
-enum { FACTOR_NONE, FACTOR_FLOAT, FACTOR_HALF, FACTOR_FIXED, FACTOR_SIGN };
+enum { FACTOR_NONE, FACTOR_FLOAT, FACTOR_HALF, FACTOR_SHORT, FACTOR_SIGN };
 template <class T> struct FactorOf { using type = int16_t; };
 template <> struct FactorOf<float> { using type = float; };
+
+// (the exponent of a fp32 2^112 times smaller -- its subnormal numbers the format's -- and the upper half of its mantissa)
+__device__ __forceinline__ int16_t short_float(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v * 0x1p-112f), m = b & 0x7fffffffu;
+  return v == v ? (int16_t)((b >> 16 & 0x8000u) | (m + 0x7ffu + (m >> 12 & 1u)) >> 12) : (int16_t)0x7fff;
+}
+__device__ __forceinline__ float short_float_value(int16_t q) {
+  const float v = __builtin_bit_cast(float, (uint32_t)(int)q << 12 & 0x87fff000u) * 0x1p112f;
+  return q == 0x7fff ? __builtin_nanf("") : v;
+}
 
 template <int FACTOR, class Q>
 __device__ __forceinline__ float factor_value(Q q, float leak) {
   if constexpr (FACTOR == FACTOR_FLOAT) return (float)q;
   if constexpr (FACTOR == FACTOR_HALF) return (float)__builtin_bit_cast(_Float16, q);
   if constexpr (FACTOR == FACTOR_SIGN) return q == 2 ? 1.f : q == 1 ? leak : 0.f;
-  return (int)q == -32768 ? __builtin_nanf("") : (float)(int)q * (1.f / 16384.f);
+  return short_float_value((int16_t)q);
 }
 
 struct LinearArgs {
@@ -163,7 +174,7 @@ __device__ __forceinline__ float activated(float z, bool keep, const LinearArgs 
   else if constexpr (ACT == ACT_NONE) factor = 2;
   else if constexpr (ACT == SCN_ACT_LEAKY) factor = z > 0 ? 2 : 1;
   else if constexpr (std::is_same<T, __bf16>::value) factor = __builtin_bit_cast(int16_t, (_Float16)slope);
-  else factor = slope == slope ? (int16_t)(int)rintf(slope * 16384.f) : -32768;
+  else factor = short_float(slope);
   if (DROP && !keep) factor = 0;
   return value;
 }
@@ -808,7 +819,7 @@ static int by_factor(const void *factor, int act, F &&f) {
   if (!factor) return f(std::integral_constant<int, FACTOR_NONE>());
   if constexpr (sizeof(T) == 4) return f(std::integral_constant<int, FACTOR_FLOAT>());
   else if (act == SCN_ACT_LEAKY) return f(std::integral_constant<int, FACTOR_SIGN>());
-  else return f(std::integral_constant<int, std::is_same<T, __bf16>::value ? FACTOR_HALF : FACTOR_FIXED>());
+  else return f(std::integral_constant<int, std::is_same<T, __bf16>::value ? FACTOR_HALF : FACTOR_SHORT>());
 }
 
 // row slices of dW: with its 64 x 64 tiles four workgroups a CU (two of the wide ones), no slice below 256 rows

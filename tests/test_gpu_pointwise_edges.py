@@ -1,0 +1,45 @@
+"""-m gpu: the pointwise operators where their results are small, masked, shared between streams or made by another kernel; against
+float64 (oracle/pointwise.py).  U and half_step as in test_gpu_pointwise."""
+import pytest
+import torch
+
+from oracle import pointwise as O
+from test_gpu_pointwise import APPROX, TYPES, U, check, half_step, rnd, run_linear
+
+pytestmark = pytest.mark.gpu
+
+
+# the stored slope, an error relative to the slope and an absolute one below its normal numbers: fp32 keeps the fp32 slope; beside fp16
+# 11 bits of mantissa down to 2^-14, half a step of its subnormal numbers 2^-26
+STORED = {"f32": (0.0, 0.0), "f16": (2.0 ** -12, 2.0 ** -26)}
+SATURATED = [("f32", "silu", -14, -6), ("f32", "gelu", -4.5, -3), ("f16", "silu", -14, -6), ("f16", "gelu", -4.5, -3)]
+
+
+@pytest.mark.parametrize("p", [0.0, 0.25])
+@pytest.mark.parametrize("N,K,M", [(3, 8, 5), (300, 35, 7), (300, 64, 40)])
+@pytest.mark.parametrize("dtype,activation,low,high", SATURATED)
+def test_gradients_of_saturated_units(gpu, dtype, activation, low, high, N, K, M, p):
+    """pre-activations where the slope is far below 1: every gradient within a bound relative to the slopes themselves.  dy is large (a scaled
+    loss), so that fp16's dz = dy slope is not lost among its subnormal numbers"""
+    t = TYPES[dtype]
+    g = torch.Generator().manual_seed(5)
+    x, w = rnd(1, N, K).to(t), (rnd(2, K, M) * 0.1 * K ** -0.5).to(t)
+    b = (low + (high - low) * torch.rand(M, generator=g, dtype=torch.float64)).to(t)
+    dy = (64 * rnd(3, N, M)).to(t)
+    rng = torch.tensor([3, 4], dtype=torch.int64, device=gpu)
+    keep = O.keep(3, 4, N, M, p) if p else None
+    got = run_linear(gpu, x, w, b, None, activation, 1, p, rng, dy)
+    X, W, B, DY = (v.double() for v in (x, w, b, dy))
+    o = O.linear(X, W, B, None, activation, 1, keep, p, DY)
+    h, (relative, absolute) = half_step(t), STORED[dtype]
+    tiny = torch.finfo(t).smallest_normal * h  # half the smallest subnormal number
+    ez = (K + 4) * U * (X.abs() @ W.abs() + B.abs())
+    # |act'' / act'| <= 5.5 over these ranges (GELU: (2 - z^2) phi over z phi + Phi; SiLU: below 1); act' itself: exponents of up to 30, each
+    # step of theirs an error of 30 U relative
+    f = o["f"].abs()
+    ef = f * (5.5 * ez + 2 * APPROX[t] + 64 * U + relative) + (absolute / (1 - p) if p == 0 else absolute / (1 - p) * keep.double())
+    edz = DY.abs() * ef + (h + 4 * U) * o["dz"].abs() + tiny / (1 - p)
+    check(got[1], o["dx"], 1.01 * ((edz + (M + 4) * U * o["dz"].abs()) @ W.abs().t() + h * o["dx"].abs() + tiny), "dx")
+    rounds = (N + 4) * U * o["dz"].abs()
+    check(got[2], o["dw"], 1.01 * (X.abs().t() @ (edz + rounds) + h * o["dw"].abs() + tiny), "dweight")
+    check(got[3], o["db"], 1.01 * ((edz + rounds).sum(0) + h * o["db"].abs() + tiny), "dbias")
