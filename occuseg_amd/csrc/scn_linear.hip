@@ -119,28 +119,43 @@ __device__ __forceinline__ floatx4 mma(const halfx8 &a, const halfx8 &b, const f
 // multiplied with; 1 / (1 - p) is applied to the sums.)  dz = dy slope is rounded to the features' type as the matrix units' operand;
 // slopes rounded to the same type would make that rounding twice, so they are kept finer:
 //   FACTOR_FLOAT  fp32 features: fp32
-//   FACTOR_HALF   bf16 features: fp16, 2^-12 of a slope
-//   FACTOR_SHORT  fp16 features: sign, 4 bits of exponent, 11 of mantissa: 2^-12 of a slope from 2^-14 to 2 (the smooth activations'
-//                 are below 1.13), 2^-26 below, where dz itself is among fp16's subnormal numbers; 0x7fff: NaN
+//   FACTOR_WIDE   bf16 features: sign, 6 bits of exponent, 9 of mantissa: 2^-10 of a slope down to 2^-60 (slopes of saturated units are
+//                 small, and bf16 holds what they make of dy), 2^-60 below
+//   FACTOR_SHORT  fp16 features: the smooth activations' slopes are below 1.13, and above -0.13, where those of saturated units are:
+//                 positive ones 3 bits of exponent and 12 of mantissa (2^-13 of a slope down to 2^-6, 2^-19 below: next to the slope's
+//                 zero), negative ones 5 and 10 (2^-11 down to 2^-33, 2^-44 below); 0x7fff: NaN
 //   FACTOR_SIGN   leaky ReLU of 16-bit features, whose slope may be any number: 2: 1, 1: leak, 0: dropped
-enum { FACTOR_NONE, FACTOR_FLOAT, FACTOR_HALF, FACTOR_SHORT, FACTOR_SIGN };
+enum { FACTOR_NONE, FACTOR_FLOAT, FACTOR_WIDE, FACTOR_SHORT, FACTOR_SIGN };
 template <class T> struct FactorOf { using type = int16_t; };
 template <> struct FactorOf<float> { using type = float; };
 
-// (the exponent of a fp32 2^112 times smaller -- its subnormal numbers the format's -- and the upper half of its mantissa)
+// (the low bits of the exponent of a fp32 2^126 times larger, which are 192 more -- the largest are NaN's -- and the upper of its mantissa)
+__device__ __forceinline__ int16_t wide_float(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, fabsf(v) * 0x1p126f), sign = __builtin_bit_cast(uint32_t, v) >> 16 & 0x8000u;
+  return (int16_t)(__builtin_elementwise_sub_sat(b, (192u << 23) - 0x2000u) >> 14 | sign);
+}
+__device__ __forceinline__ float wide_float_value(int16_t q) {
+  const float v = __builtin_bit_cast(float, ((uint32_t)(int)q << 14 & 0x9fffc000u) | 0x60000000u) * 0x1p-126f;
+  return q == 0 ? 0.f : v;
+}
+// (the low bits of the exponent of a fp32 2^120 or 2^93 times smaller -- its subnormal numbers are the format's -- and the upper of its
+// mantissa)
 __device__ __forceinline__ int16_t short_float(float v) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, v * 0x1p-112f), m = b & 0x7fffffffu;
-  return v == v ? (int16_t)((b >> 16 & 0x8000u) | (m + 0x7ffu + (m >> 12 & 1u)) >> 12) : (int16_t)0x7fff;
+  const bool negative = v < 0;
+  const uint32_t b = __builtin_bit_cast(uint32_t, fabsf(v) * (negative ? 0x1p-93f : 0x1p-120f));
+  const int shift = negative ? 13 : 11;
+  return v == v ? (int16_t)((b + (1u << shift >> 1)) >> shift | (negative ? 0x8000u : 0u)) : (int16_t)0x7fff;
 }
 __device__ __forceinline__ float short_float_value(int16_t q) {
-  const float v = __builtin_bit_cast(float, (uint32_t)(int)q << 12 & 0x87fff000u) * 0x1p112f;
+  const bool negative = q < 0;
+  const float v = __builtin_bit_cast(float, ((uint32_t)q & 0x7fffu) << (negative ? 13 : 11)) * (negative ? -0x1p93f : 0x1p120f);
   return q == 0x7fff ? __builtin_nanf("") : v;
 }
 
 template <int FACTOR, class Q>
 __device__ __forceinline__ float factor_value(Q q, float leak) {
   if constexpr (FACTOR == FACTOR_FLOAT) return (float)q;
-  if constexpr (FACTOR == FACTOR_HALF) return (float)__builtin_bit_cast(_Float16, q);
+  if constexpr (FACTOR == FACTOR_WIDE) return wide_float_value((int16_t)q);
   if constexpr (FACTOR == FACTOR_SIGN) return q == 2 ? 1.f : q == 1 ? leak : 0.f;
   return short_float_value((int16_t)q);
 }
@@ -173,7 +188,7 @@ __device__ __forceinline__ float activated(float z, bool keep, const LinearArgs 
   if constexpr (sizeof(T) == 4) factor = slope;
   else if constexpr (ACT == ACT_NONE) factor = 2;
   else if constexpr (ACT == SCN_ACT_LEAKY) factor = z > 0 ? 2 : 1;
-  else if constexpr (std::is_same<T, __bf16>::value) factor = __builtin_bit_cast(int16_t, (_Float16)slope);
+  else if constexpr (std::is_same<T, __bf16>::value) factor = wide_float(slope);
   else factor = short_float(slope);
   if (DROP && !keep) factor = 0;
   return value;
@@ -819,7 +834,7 @@ static int by_factor(const void *factor, int act, F &&f) {
   if (!factor) return f(std::integral_constant<int, FACTOR_NONE>());
   if constexpr (sizeof(T) == 4) return f(std::integral_constant<int, FACTOR_FLOAT>());
   else if (act == SCN_ACT_LEAKY) return f(std::integral_constant<int, FACTOR_SIGN>());
-  else return f(std::integral_constant<int, std::is_same<T, __bf16>::value ? FACTOR_HALF : FACTOR_SHORT>());
+  else return f(std::integral_constant<int, std::is_same<T, __bf16>::value ? FACTOR_WIDE : FACTOR_SHORT>());
 }
 
 // row slices of dW: with its 64 x 64 tiles four workgroups a CU (two of the wide ones), no slice below 256 rows
