@@ -14,7 +14,7 @@ def act(z, activation, leakiness=1.0):
         s = torch.special.expit(z)
         return z * s, s * (1 + z * (1 - s))
     if activation == GELU:
-        cdf = torch.special.ndtr(z)
+        cdf = torch.erfc(-z * math.sqrt(0.5)) / 2  # (torch's ndtr is within 2^-55 of 1, not of itself)
         return z * cdf, cdf + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
     slope = torch.where(z > 0, torch.ones_like(z), torch.full_like(z, float(leakiness)))
     return z * slope, slope
