@@ -116,8 +116,8 @@ __device__ __forceinline__ floatx4 mma(const halfx8 &a, const halfx8 &b, const f
 }
 
 // What the backward pass needs of activation and mask, one value per output: the slope, 0 for a dropped element.  (dy slope is what is
-// multiplied with; 1 / (1 - p) is applied to the sums.)  dz = dy slope is rounded to the features' type as the matrix units' operand;
-// slopes rounded to the same type would make that rounding twice, so they are kept finer:
+// multiplied with; 1 / (1 - p) is applied to the sums.)  dz = dy slope is the matrix units' operand, 16-bit features' in two parts (split,
+// below); a slope's own rounding is all that it loses, so slopes are kept finer than the features:
 //   FACTOR_FLOAT  fp32 features: fp32
 //   FACTOR_WIDE   bf16 features: sign, 6 bits of exponent, 9 of mantissa: 2^-10 of a slope down to 2^-60 (slopes of saturated units are
 //                 small, and bf16 holds what they make of dy), 2^-60 below
@@ -158,6 +158,18 @@ __device__ __forceinline__ float factor_value(Q q, float leak) {
   if constexpr (FACTOR == FACTOR_WIDE) return wide_float_value((int16_t)q);
   if constexpr (FACTOR == FACTOR_SIGN) return q == 2 ? 1.f : q == 1 ? leak : 0.f;
   return short_float_value((int16_t)q);
+}
+
+// z of 16-bit features as two operands, z rounded and what that lost, whose products are added one behind the other: what is lost is the
+// square of a rounding (fp16: and what lies below its subnormal numbers).  One operand alone doubles the variance of the gradients' own
+// rounding (bf16 dx and dW off by 2.4e-3 instead of 1.7e-3, relative), and the matrix pipe waits for memory either way: 177,001 x 128 to
+// 512, bf16, GELU, dx 94 us with one and with two, dW 108 and 109.  (Where rounding would give infinity: the largest number, and the rest
+// beside it; infinity and NaN are in the rest.)
+template <class T>
+__device__ __forceinline__ void split(float z, T &rounded, T &rest) {
+  constexpr float most = std::is_same<T, __bf16>::value ? 0x1.fep127f : 65504.f;
+  rounded = (T)__builtin_amdgcn_fmed3f(z, -most, most);
+  rest = (T)(z - (float)rounded);
 }
 
 struct LinearArgs {
@@ -220,7 +232,7 @@ __global__ void __launch_bounds__(64 * lin_waves(NT, STAY), NT == 8 || !STAY ? 3
   constexpr int V = Elem<T>::V, KG = 4 * V;
   constexpr bool PACKED = lin_packed(MODE, sizeof(T));
   constexpr int PC = lin_piece(NT), PITCH = PACKED ? PC + 8 : PC + 4, LPR = PC / V, RPI = 64 / LPR;  // planes, lanes a row, rows an instruction of a piece
-  constexpr bool FACTORS = MODE == 1 && X != FACTOR_NONE;
+  constexpr bool FACTORS = MODE == 1 && X != FACTOR_NONE, SPLIT = FACTORS && sizeof(T) == 2;
   using F = typename Frag<T>::type;
   using Q = typename FactorOf<T>::type;
   extern __shared__ char smem[];
@@ -405,12 +417,19 @@ __global__ void __launch_bounds__(64 * lin_waves(NT, STAY), NT == 8 || !STAY ? 3
       constexpr int G = sizeof(v) / sizeof(v[0]);
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        F b[2], w[NT];
+        F b[2], rest[2], w[NT];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          if constexpr (FACTORS)
+          if constexpr (FACTORS) {
+            Pack<T, V> r;
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[i][u].v[j] = (T)((float)v[i][u].v[j] * factor_value<X>(f[i][u].v[j], a.leak));
+            for (int j = 0; j < V; ++j) {
+              const float z = (float)v[i][u].v[j] * factor_value<X>(f[i][u].v[j], a.leak);
+              if constexpr (SPLIT) split(z, v[i][u].v[j], r.v[j]);
+              else v[i][u].v[j] = (T)z;
+            }
+            if constexpr (SPLIT) __builtin_memcpy(&rest[u], &r, 16);
+          }
           __builtin_memcpy(&b[u], &v[i][u], 16);
         }
 #pragma unroll
@@ -426,9 +445,12 @@ __global__ void __launch_bounds__(64 * lin_waves(NT, STAY), NT == 8 || !STAY ? 3
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) acc[u][t] = mma(w[t], b[u], acc[u][t]);
+            for (int u = 0; u < 2; ++u) {
+              acc[u][t] = mma(w[t], b[u], acc[u][t]);
+              if constexpr (SPLIT) acc[u][t] = mma(w[t], rest[u], acc[u][t]);
+            }
         }
-        if (NT == 8) __builtin_amdgcn_sched_barrier(0);  // (one k-group's weights in registers at a time)
+        if (NT == 8 || SPLIT) __builtin_amdgcn_sched_barrier(0);  // (one k-group's operands in registers at a time)
       }
     };
     auto batch = [&](auto count, auto whole, int g, const F *wg) __attribute__((always_inline)) {
@@ -601,12 +623,9 @@ __global__ void __launch_bounds__(256, 2) k_linear_dw(DwArgs a) {
   const int ci0 = tile / a.tiles_o * 64 * TI, co0 = tile % a.tiles_o * 64;
   const bool bias = a.want_bias && ci0 == 0;
   const int64_t r0 = slice * a.slice_rows, r1 = min(r0 + a.slice_rows, a.N);
-  const int ci = ci0 + 4 * li, co = co0 + 4 * li, no = a.Co - co;
   // a step's rows from scalar addresses, a lane's part of them from 32-bit offsets
   const T *px = (const T *)a.x + ci0, *pd = (const T *)a.dy + co0;
   const Q *pf = (const Q *)a.factor + co0;
-  const int lr = F32 ? lq : lq * RE;  // a lane's first row (fp32: a load of four whole rows; 16-bit: a lane's eight rows)
-  const unsigned ox = (unsigned)(lr * (int)a.ldx + 4 * li), od = (unsigned)(lr * (int)a.ld_dy + 4 * li), of = (unsigned)(lr * a.Co + 4 * li);
   int64_t inside = min(rows_inside(a.N, a.ldx, a.Ci, ci0 + 64 * TI), rows_inside(a.N, a.ld_dy, a.Co, co0 + 64));
   if (FACTOR != FACTOR_NONE) inside = min(inside, rows_inside(a.N, a.Co, a.Co, co0 + 64));
   inside = min(inside, r1);
@@ -622,6 +641,11 @@ __global__ void __launch_bounds__(256, 2) k_linear_dw(DwArgs a) {
     Pack<Q, 4> vf[RE];
     const T *p = px + r * a.ldx, *d = pd + r * a.ld_dy;
     const Q *q = pf + r * a.Co;
+    int l = lane;
+    if (!WHOLE) asm volatile("" : "+v"(l));  // (nothing of these steps is kept in registers through the loop of the whole ones)
+    const int lr = F32 ? l >> 4 : (l >> 4) * RE;  // a lane's first row (fp32: a load of four whole rows; 16-bit: a lane's eight rows)
+    const int lc = 4 * (l & 15), ci = ci0 + lc, no = a.Co - co0 - lc;
+    const unsigned ox = (unsigned)(lr * (int)a.ldx + lc), od = (unsigned)(lr * (int)a.ld_dy + lc), of = (unsigned)(lr * a.Co + lc);
 #pragma unroll
     for (int e = 0; e < RE; ++e) {
       const bool in = r + ES * e + lr < r1;
@@ -654,22 +678,29 @@ __global__ void __launch_bounds__(256, 2) k_linear_dw(DwArgs a) {
             acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[i / 4][e].v[i & 3], z[j], acc[i][j], 0, 0, 0);
       }
     } else {
-      F fd[4];
+      F fx[4 * TI];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int i = 0; i < 4 * TI; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) fx[i][e] = vx[i / 4][e].v[i & 3];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        F fd, rest;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float z = dz(e, j);
-          sums[j] += z;  // (of the values that the matrix units' operand rounds)
-          fd[j][e] = (T)z;
+          sums[j] += z;
+          T value = (T)z, low = (T)0.f;
+          if constexpr (FACTOR != FACTOR_NONE) split(z, value, low);
+          fd[e] = value;
+          rest[e] = low;
         }
 #pragma unroll
-      for (int i = 0; i < 4 * TI; ++i) {
-        F fx;
+        for (int i = 0; i < 4 * TI; ++i) acc[i][j] = mma(fx[i], fd, acc[i][j]);
+        if constexpr (FACTOR != FACTOR_NONE)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) fx[e] = vx[i / 4][e].v[i & 3];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mma(fx, fd[j], acc[i][j]);
+          for (int i = 0; i < 4 * TI; ++i) acc[i][j] = mma(fx[i], rest, acc[i][j]);
+        if (TI == 2) __builtin_amdgcn_sched_barrier(0);  // (one column tile's operands in registers at a time)
       }
     }
   };
@@ -707,6 +738,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_dw(DwArgs a) {
   }
   if (wave != 0) return;
   float *slab = a.slab + (int64_t)slice * a.Ci * a.Co;
+  const int co = co0 + 4 * li, no = a.Co - co;
 #pragma unroll
   for (int i = 0; i < 4 * TI; ++i)
 #pragma unroll

@@ -40,8 +40,51 @@ def test_gradients_of_saturated_units(gpu, dtype, activation, low, high, N, K, M
     # exponents of up to 52, rounded three times
     f = o["f"].abs()
     ef = f * (9 * ez + 2 * APPROX[t] + 160 * U + relative) + (absolute / (1 - p) if p == 0 else absolute / (1 - p) * keep.double())
-    edz = DY.abs() * ef + (h + 4 * U) * o["dz"].abs() + tiny / (1 - p)
-    check(got[1], o["dx"], 1.01 * ((edz + (M + 4) * U * o["dz"].abs()) @ W.abs().t() + h * o["dx"].abs() + tiny), "dx")
-    rounds = (N + 4) * U * o["dz"].abs()
+    # dz itself: two operands of the type, the second a rounding of at most h of it, rounded in turn
+    edz = DY.abs() * ef + (2 * h * h + 4 * U) * o["dz"].abs() + tiny / (1 - p)
+    check(got[1], o["dx"], 1.01 * ((edz + (2 * M + 4) * U * o["dz"].abs()) @ W.abs().t() + h * o["dx"].abs() + tiny), "dx")
+    rounds = (2 * N + 4) * U * o["dz"].abs()
     check(got[2], o["dw"], 1.01 * (X.abs().t() @ (edz + rounds) + h * o["dw"].abs() + tiny), "dweight")
     check(got[3], o["db"], 1.01 * ((edz + rounds).sum(0) + h * o["db"].abs() + tiny), "dbias")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("N,K,M", [(300, 64, 1), (1, 64, 300), (700, 130, 1), (9, 20, 3)])
+@pytest.mark.parametrize("activation,leak", [("silu", 1), ("gelu", 1), ("leaky_relu", 0.333)])
+def test_gradients_lose_one_rounding(gpu, dtype, N, K, M, activation, leak):
+    """sums of one or a few terms: the operand's rounding would show beside the result's"""
+    t = TYPES[dtype]
+    x, w, b, dy = rnd(11, N, K).to(t), (rnd(12, K, M) * K ** -0.5).to(t), (0.1 * rnd(13, M)).to(t), rnd(14, N, M).to(t)
+    got = run_linear(gpu, x, w, b, None, activation, leak, 0.0, None, dy)
+    X, W, B, DY = (v.double() for v in (x, w, b, dy))
+    o = O.linear(X, W, B, None, activation, leak, None, 0.0, DY)
+    h = half_step(t)
+    tiny = torch.finfo(t).smallest_normal * h
+    ez = (K + 4) * U * (X.abs() @ W.abs() + B.abs())
+    if activation == "leaky_relu":
+        assert (o["z"].abs() > ez).all()  # (on one side of the kink; the slope is the caller's fp32 number)
+        ef = U * o["f"].abs()
+    else:  # stored slopes: fp16 2^-13 of positive ones, 2^-11 of negative ones, 2^-19 where they are below 2^-6
+        relative, absolute = (2.0 ** -10, 0.0) if dtype == "bf16" else (2.0 ** -11, 2.0 ** -19)
+        ef = 0.8 * ez + (8 * U + APPROX[t]) * (1 + o["z"].abs()) + relative * o["f"].abs() + absolute
+        if dtype == "f16":
+            ef = torch.where(o["f"] > 2.0 ** -5, ef - (2.0 ** -11 - 2.0 ** -13) * o["f"] - absolute, ef)
+    edz = DY.abs() * ef + (2 * h * h + 4 * U) * o["dz"].abs() + tiny
+    check(got[1], o["dx"], 1.01 * ((edz + (2 * M + 4) * U * o["dz"].abs()) @ W.abs().t() + h * o["dx"].abs() + tiny), "dx")
+    rounds = (2 * N + 4) * U * o["dz"].abs()
+    check(got[2], o["dw"], 1.01 * (X.abs().t() @ (edz + rounds) + h * o["dw"].abs() + tiny), "dweight")
+    check(got[3], o["db"], 1.01 * ((edz + rounds).sum(0) + h * o["db"].abs() + tiny), "dbias")
+
+
+def test_gradients_next_to_the_largest_number(gpu):
+    """fp16: dy 60,000 times a slope above 1 leaves the type, the products with small weights and rows do not"""
+    N, K, M = 40, 16, 8
+    x, w = (rnd(1, N, K) * 2.0 ** -8).half(), (rnd(2, K, M) * 2.0 ** -6).half()
+    b = torch.full((M,), 1.4).half()
+    dy = torch.full((N, M), 60000.0).half()
+    got = run_linear(gpu, x, w, b, None, "gelu", 1, 0.0, None, dy)
+    o = O.linear(x.double(), w.double(), b.double(), None, "gelu", 1, None, 0.0, dy.double())
+    assert (o["dz"] > 65504).all() and float(o["dx"].abs().max()) < 65504 and float(o["dw"].abs().max()) < 65504
+    e = (2.0 ** -13 + 2 * APPROX[torch.float16] + 64 * U) * o["dz"]  # stored slope, its computation; dz's second operand is exact
+    check(got[1], o["dx"], 1.01 * (e @ w.double().abs().t() + 2.0 ** -11 * o["dx"].abs() + 2.0 ** -25), "dx")
+    check(got[2], o["dw"], 1.01 * (x.double().abs().t() @ e + 2.0 ** -11 * o["dw"].abs() + 2.0 ** -25), "dweight")
