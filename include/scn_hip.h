@@ -497,7 +497,7 @@ size_t scn_linear_forward_temp_bytes(int64_t N, int n_in, int n_out, int dtype);
 int scn_linear_forward(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_res,
                        void *y, void *factor, int64_t N, int n_in, int n_out, int act, double leakiness, double p,
                        const int64_t *rng, int dtype, void *temp, size_t temp_bytes, void *stream);
-/* d_x = (d_y factor) weight^T; factor NULL: ones.  d_y rows at ld_dy elements */
+/* d_x = (d_y factor) weight^T; factor NULL: ones.  d_y factor is 0 where factor is, infinite d_y too.  d_y rows at ld_dy elements */
 int scn_linear_dinput(const void *d_y, int64_t ld_dy, const void *factor, const void *weight, void *d_x, int64_t N, int n_in,
                       int n_out, int act, double leakiness, double p, int dtype, void *stream);
 /* d_weight = x^T (d_y factor), d_bias = column sums of (d_y factor) (NULL: not wanted), of `dtype`, assigned; partial sums are

@@ -1,6 +1,6 @@
 // 1x1 convolution with its epilogue, y = residual + drop(act(x W + b)), its gradients, and dropout alone (gfx950).
 //
-//   backward:  f = act'(x W + b), 0 where dropped, left by the forward pass;  dz = dy f / (1 - p);
+//   backward:  f = act'(x W + b), 0 where dropped, left by the forward pass;  dz = dy f / (1 - p), 0 where f is 0;
 //              dx = dz W^T;  dW = x^T dz;  db = column sums of dz
 //
 // Sites are many (up to 600k) and planes few (16 to 512), so the products are HBM bound but for the widest: 2 n_in n_out flops for
@@ -135,8 +135,7 @@ __device__ __forceinline__ int16_t wide_float(float v) {
   return (int16_t)(__builtin_elementwise_sub_sat(b, (192u << 23) - 0x2000u) >> 14 | sign);
 }
 __device__ __forceinline__ float wide_float_value(int16_t q) {
-  const float v = __builtin_bit_cast(float, ((uint32_t)(int)q << 14 & 0x9fffc000u) | 0x60000000u) * 0x1p-126f;
-  return q == 0 ? 0.f : v;
+  return __builtin_bit_cast(float, ((uint32_t)(int)q << 14 & 0x9fffc000u) | 0x60000000u) * 0x1p-126f;
 }
 // (the low bits of the exponent of a fp32 2^120 or 2^93 times smaller -- its subnormal numbers are the format's -- and the upper of its
 // mantissa)
@@ -152,12 +151,14 @@ __device__ __forceinline__ float short_float_value(int16_t q) {
   return q == 0x7fff ? __builtin_nanf("") : v;
 }
 
+// dy times the slope; 0 where that is 0, whatever dy is there: infinity and NaN in dropped places stay there
 template <int FACTOR, class Q>
-__device__ __forceinline__ float factor_value(Q q, float leak) {
-  if constexpr (FACTOR == FACTOR_FLOAT) return (float)q;
-  if constexpr (FACTOR == FACTOR_WIDE) return wide_float_value((int16_t)q);
-  if constexpr (FACTOR == FACTOR_SIGN) return q == 2 ? 1.f : q == 1 ? leak : 0.f;
-  return short_float_value((int16_t)q);
+__device__ __forceinline__ float times_factor(float dy, Q q, float leak) {
+  if constexpr (FACTOR == FACTOR_FLOAT) return q == 0 ? 0.f : dy * (float)q;
+  if constexpr (FACTOR == FACTOR_WIDE) return q == 0 ? 0.f : dy * wide_float_value((int16_t)q);
+  float slope = q == 2 ? 1.f : q == 1 ? leak : 0.f;
+  if constexpr (FACTOR == FACTOR_SHORT) slope = short_float_value((int16_t)q);
+  return slope == 0 ? 0.f : dy * slope;
 }
 
 // z of 16-bit features as two operands, z rounded and what that lost, whose products are added one behind the other: what is lost is the
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(64 * lin_waves(NT, STAY), NT == 8 || !STAY ? 3
             Pack<T, V> r;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-              const float z = (float)v[i][u].v[j] * factor_value<X>(f[i][u].v[j], a.leak);
+              const float z = times_factor<X>((float)v[i][u].v[j], f[i][u].v[j], a.leak);
               if constexpr (SPLIT) split(z, v[i][u].v[j], r.v[j]);
               else v[i][u].v[j] = (T)z;
             }
@@ -660,9 +661,8 @@ __global__ void __launch_bounds__(256, 2) k_linear_dw(DwArgs a) {
       if (!WHOLE) __builtin_amdgcn_sched_barrier(0);  // (a row at a time: nothing to gain, and fewer registers)
     }
     auto dz = [&](int e, int j) __attribute__((always_inline)) {
-      float v = (float)vd[e].v[j];
-      if constexpr (FACTOR != FACTOR_NONE) v *= factor_value<FACTOR>(vf[e].v[j], a.leak);
-      return v;
+      if constexpr (FACTOR != FACTOR_NONE) return times_factor<FACTOR>((float)vd[e].v[j], vf[e].v[j], a.leak);
+      return (float)vd[e].v[j];
     };
     if constexpr (F32) {
 #pragma unroll

@@ -88,3 +88,31 @@ def test_gradients_next_to_the_largest_number(gpu):
     e = (2.0 ** -13 + 2 * APPROX[torch.float16] + 64 * U) * o["dz"]  # stored slope, its computation; dz's second operand is exact
     check(got[1], o["dx"], 1.01 * (e @ w.double().abs().t() + 2.0 ** -11 * o["dx"].abs() + 2.0 ** -25), "dx")
     check(got[2], o["dw"], 1.01 * (x.double().abs().t() @ e + 2.0 ** -11 * o["dw"].abs() + 2.0 ** -25), "dweight")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("activation,leak", [("silu", 1), ("gelu", 1), ("leaky_relu", 1), ("leaky_relu", 0.25), ("leaky_relu", 0)])
+@pytest.mark.parametrize("N,K,M", [(3, 5, 4), (200, 70, 33), (300, 130, 72)])
+def test_bad_gradients_of_dropped_elements_stay_there(gpu, dtype, activation, leak, N, K, M):
+    """as a dropout layer's do: the gradients are those of zeros in their places, bit for bit.  A bad one that is kept reaches its row of dx
+    and its column of dW and db"""
+    t = TYPES[dtype]
+    x, w, b, dy = rnd(21, N, K).to(t), (rnd(22, K, M) * K ** -0.5).to(t), (0.1 * rnd(23, M)).to(t), rnd(24, N, M).to(t)
+    rng = torch.tensor([6, 7], dtype=torch.int64, device=gpu)
+    keep = O.keep(6, 7, N, M, 0.5)
+    clean = torch.where(keep, dy, torch.zeros_like(dy))
+    bad = torch.full_like(dy, float("inf"))
+    bad[::2] = float("nan")
+    bad[:, ::3] = -float("inf")
+    want = run_linear(gpu, x, w, b, None, activation, leak, 0.5, rng, clean)
+    got = run_linear(gpu, x, w, b, None, activation, leak, 0.5, rng, torch.where(keep, dy, bad))
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    if activation == "leaky_relu" and leak == 0:
+        return  # (a ReLU's slope may be 0 where nothing was dropped)
+    r, c = [int(i) for i in keep.nonzero()[len(keep.nonzero()) // 2]]
+    clean[r, c] = float("nan")
+    got = run_linear(gpu, x, w, b, None, activation, leak, 0.5, rng, clean)
+    rows, columns = torch.arange(N) != r, torch.arange(M) != c
+    assert got[1][r].isnan().all() and torch.equal(got[1][rows], want[1][rows])
+    assert got[2][:, c].isnan().all() and torch.equal(got[2][:, columns], want[2][:, columns])
+    assert got[3][c].isnan() and torch.equal(got[3][columns], want[3][columns])
