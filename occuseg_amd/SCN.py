@@ -370,7 +370,7 @@ class Metadata_3(object):
         self._occ = None          # (scn_occ_box, buffer) between scn_occ_chain and scn_batch_build_occ
         self._grid_status = []    # (device [N, error flag] of a grid built without read-back, the N it was built for)
         self.nSamples = None      # largest sample index of the batch + 1, once somebody has needed or found it
-        self._sample_offsets = {} # spatial size -> int64 [nSamples + 1] on the device, see sampleOffsets
+        self._sample_offsets = {} # spatial size -> (int64 [nSamples + 1] on the device, the stream it was made on, event), see sampleOffsets
 
     def setNormalGuideScale(self, s):
         self.normal_guide_scale = int(s)
@@ -772,19 +772,30 @@ class Metadata_3(object):
 
     def sampleOffsets(self, spatialSize):
         """int64 [samples + 1] on the device: the sites of sample s are rows offsets[s] to offsets[s + 1] of the scale's
-        features.  Made once per batch and scale; the first call of a batch may read the number of samples back."""
+        features.  Made once per batch and scale, on the stream that asks first (it has to be behind the batch's build, as for any
+        layer); others that ask wait for it.  The first call of a batch may read the number of samples back.  A capture records no
+        such wait: torch.cuda.graph synchronises the device before it begins."""
         key = _size_key(spatialSize)
-        offsets = self._sample_offsets.get(key)
-        if offsets is None:
+        made = self._sample_offsets.get(key)
+        if made is None:
             g = self.grids[key]
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("occuseg_amd.SCN.sampleOffsets: run the layer once on this batch before capturing it (the number "
                                    "of samples may have to be read back)")
-            if self.nSamples is None:
-                self.nSamples = (int(g.keys[-1].item()) >> 31) + 1 if g.n else 1
-            offsets = torch.empty(self.nSamples + 1, dtype=torch.int64, device=g.keys.device)
-            check(_lib_().scn_sample_offsets(ptr(g.keys), g.n, self.nSamples, ptr(offsets), stream()))
-            self._sample_offsets[key] = offsets
+            with _on(g.keys):
+                if self.nSamples is None:
+                    self.nSamples = (int(g.keys[-1].item()) >> 31) + 1 if g.n else 1
+                offsets = torch.empty(self.nSamples + 1, dtype=torch.int64, device=g.keys.device)
+                check(_lib_().scn_sample_offsets(ptr(g.keys), g.n, self.nSamples, ptr(offsets), stream()))
+                event = torch.cuda.Event()
+                event.record()
+                made = self._sample_offsets[key] = offsets, stream(), event
+        offsets, made_on, event = made
+        with _on(offsets):
+            if stream() != made_on and not torch.cuda.is_current_stream_capturing():
+                cur = torch.cuda.current_stream()
+                cur.wait_event(event)
+                offsets.record_stream(cur)  # (the batch may be dropped while that stream's kernels read them)
         return offsets
 
     # -- rulebooks -----------------------------------------------------------

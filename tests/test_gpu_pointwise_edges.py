@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import pointwise as O
-from test_gpu_pointwise import APPROX, TYPES, U, check, half_step, rnd, run_linear
+from test_gpu_pointwise import APPROX, TYPES, U, batch_tensor, check, half_step, rnd, run_linear
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +116,29 @@ def test_bad_gradients_of_dropped_elements_stay_there(gpu, dtype, activation, le
     assert got[1][r].isnan().all() and torch.equal(got[1][rows], want[1][rows])
     assert got[2][:, c].isnan().all() and torch.equal(got[2][:, columns], want[2][:, columns])
     assert got[3][c].isnan() and torch.equal(got[3][columns], want[3][columns])
+
+
+def test_sample_offsets_on_several_streams(gpu):
+    """the stream that asks first makes them behind its own work; another, ordered behind the batch's build alone, waits for them and leaves
+    the memory to itself until it is through"""
+    import occuseg_amd.sparseconvnet as scn
+    lengths = [900, 0, 333, 1]
+    x = rnd(31, sum(lengths), 16).float().to(gpu)
+    module = scn.GroupNormSiLU(16, 4).to(gpu)
+    with torch.no_grad():
+        want = module(batch_tensor(gpu, scn, x, lengths)).features.clone()
+        for turn in range(3):
+            inp = batch_tensor(gpu, scn, x, lengths)
+            first, second = torch.cuda.Stream(), torch.cuda.Stream()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(first):
+                torch.cuda._sleep(20000000)
+                a = module(inp).features
+                behind = torch.cuda.Event()
+                behind.record()
+            with torch.cuda.stream(second):
+                b = module(inp).features
+            early = not behind.query()
+            inp.metadata._sample_offsets.clear()
+            torch.cuda.synchronize()
+            assert early and torch.equal(a, want) and torch.equal(b, want), turn
