@@ -541,9 +541,16 @@ static GnArgs gn_args(const int64_t *offsets, int64_t N, int C, int G, int64_t S
 }
 static int64_t gn_chunks(const GnArgs &a) { return (a.N >> a.shift) + a.S; }
 
-// (a sample has at most N sites: whatever the lengths are, a group's values fit the registers; many samples of a few sites each would
-// be as many workgroups with next to nothing to do)
-static bool gn_small(int64_t N, int C, int G, int64_t S) { return N * (C / G) <= 1024 * GN_SMALL_PER && S * G <= 4096; }
+// The one-launch path, by what was measured on the device (fp32; one launch / three, which cost the host some 5 us more):
+//   at most 512 workgroups, two a CU: 1024 sites x 512 planes in groups of one, 4 samples: 34 / 12 us; x 128: 9.6 / 10.3
+//   values a workgroup, on average: groups of one, 4 groups, 1 sample: 8192 sites 8.3 / 10.3 us, 16,384 11.7 / 10.3
+//   elements in all, a group of fewer than four planes as four (a row of a group costs its cache line however little of it is wanted):
+//   groups of one, 4 samples: 4096 sites x 32 6.2 / 10.4 us, 32,768 x 32 16.7 / 11.3, 32,768 x 1024 417 / 98
+// and, as one sample may have all N sites, a group's values fit the registers whatever the lengths are.
+static bool gn_small(int64_t N, int C, int G, int64_t S) {
+  const int64_t cpg = C / G, values = N * cpg;
+  return values <= 1024 * GN_SMALL_PER && S * G <= 512 && values <= S * 8192 && N * G * (cpg < 4 ? 4 : cpg) <= 1 << 20;
+}
 
 template <class T, int V>
 static int gn_forward(const void *x, void *y, float *stats, GnArgs a, const float *weight, const float *bias, double eps, int act,

