@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(256) k_linear_transpose(const T *w, T *out, in
 
 // Up to R rows (a serving loop's single sites): bound by one trip to memory for the weights, which the tiles above would make with a
 // few workgroups in many steps.  A workgroup has 16 output planes; its threads share out the reduction, 16 bytes of a weight row
-// each, and join in the wave, then through LDS.
+// each, and join in the wave, then through LDS: another order of additions than that of the tiles, so a row's last bits may differ.
 template <class T, int R, int ACT>
 __global__ void __launch_bounds__(1024) k_linear_few(LinearArgs a) {
   constexpr int V = Elem<T>::V, LC = 16 / V, PHASES = 1024 / LC;

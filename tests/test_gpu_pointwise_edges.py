@@ -150,3 +150,28 @@ def test_group_norm_where_one_launch_ends(gpu, lengths, C, groups, dtype):
     dy, w, b = rnd(44, N, C).to(t), (1 + 0.2 * rnd(45, C)).float(), (0.2 * rnd(46, C)).float()
     args = (x, lengths, groups, w, b, 1e-4, "silu", 1, dy)
     check_group_norm(run_group_norm(gpu, *args), *args, "one launch or three")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("K,M", [(7, 3), (100, 130), (448, 448)])
+def test_linear_of_few_rows_and_of_more(gpu, K, M, dtype):
+    """up to four rows are another kernel's, with an order of summation of its own: the bits of a row depend on which of the two it was, and
+    on nothing else; both are within the roundings of K products and of what follows them"""
+    from occuseg_amd import SCN
+    t = TYPES[dtype]
+    x, w, b, res = rnd(51, 300, K).to(t), (rnd(52, K, M) * K ** -0.5).to(t), (0.1 * rnd(53, M)).to(t), rnd(54, 300, M).to(t)
+    on = [v.to(gpu) for v in (x, w, b, res)]
+    o = O.linear(x.double(), w.double(), b.double(), res.double(), "gelu", 1, None, 0.0)
+    ez = (K + 4) * U * (x.double().abs() @ w.double().abs() + b.double().abs())
+    bound = 1.13 * ez + (8 * U + APPROX[t]) * (o["z"].abs() + 1) + 4 * U * (o["value"].abs() + o["y"].abs()) + half_step(t) * o["y"].abs()
+
+    def run(n):
+        y, factor = on[0].new_empty(0), torch.empty(0, dtype=SCN.factor_dtype(on[0]), device=gpu)
+        SCN.FusedNetworkInNetwork_updateOutput(on[0][:n], y, on[1], on[2], on[3][:n], "gelu", 1, 0.0, None, factor)
+        check(y, o["y"][:n], 1.01 * bound[:n], "%d rows" % n)
+        return y, factor
+
+    for sizes in ((4, 1, 2, 3), (300, 5, 17, 33, 100)):
+        whole = run(sizes[0])
+        for n in sizes[1:]:
+            assert all(torch.equal(a[:n], c) for a, c in zip(whole, run(n))), n
