@@ -43,8 +43,14 @@ class _Random(Module):
     """a module that draws: the buffer `rng_state` = (seed, offset), int64 [2].  The seed comes from torch's CPU generator when the
     module is made; every training forward pass uses one offset.  The counting happens on the device, so a pass captured into a
     graph draws a new mask at every replay.  Ranks of a data-parallel job that are seeded alike draw alike: `reseed` them.  A forward
-    pass that is run again for its gradients (activation checkpointing) draws again: hand it `rng`.  A state_dict without the
-    buffer (of a NetworkInNetwork) leaves it as it is."""
+    pass that is run again for its gradients (activation checkpointing) draws again: hand it `rng`.  A copy of a module draws what
+    its original draws until it is reseeded.  A state_dict without the buffer (of a NetworkInNetwork) leaves it as it is; that of a
+    module that never draws (probability 0) is without it, and a NetworkInNetwork loads it."""
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        Module._save_to_state_dict(self, destination, prefix, keep_vars)
+        if not self.p:
+            destination.pop(prefix + "rng_state", None)
 
     def _load_from_state_dict(self, state_dict, prefix, *args):
         state_dict.setdefault(prefix + "rng_state", self.rng_state)

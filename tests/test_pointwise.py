@@ -141,3 +141,15 @@ def test_group_norm_of_few_sites_needs_no_workspace():
         assert temp(*few) == 0, few
     for many in ((32768, 1024, 1024, 1), (1024, 448, 32, 1), (256, 1024, 512, 4), (32768, 32, 32, 4), (16384, 64, 32, 4), (100, 8, 2, 512)):
         assert temp(*many) > 0, many
+
+
+def test_plain_layer_takes_the_parameters_of_a_fused_one_without_dropout():
+    import occuseg_amd.sparseconvnet as scn
+    plain, fused = scn.NetworkInNetwork(5, 3, True), scn.FusedNetworkInNetwork(5, 3, True, "silu")
+    torch.nn.Sequential(plain).load_state_dict(torch.nn.Sequential(fused).state_dict())
+    assert torch.equal(plain.weight, fused.weight)
+    # and one that was saved with its state
+    old = dict(fused.state_dict(), rng_state=torch.tensor([8, 9]))
+    other = scn.FusedNetworkInNetwork(5, 3, True, "silu")
+    other.load_state_dict(old)
+    assert torch.equal(other.weight, fused.weight) and other.rng_state.tolist() == [8, 9]
