@@ -2059,6 +2059,7 @@ def rng_take(state):
     used = torch.empty(2, dtype=torch.int64, device=state.device)
     with _on(state):
         check(_lib_().scn_rng_take(ptr(_rng("rng_take", state, state)), ptr(used), stream()))
+    torch.autograd.graph.increment_version(state)  # (a backward pass that saved it as its `rng` must not take the next one)
     return used
 
 

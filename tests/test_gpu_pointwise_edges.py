@@ -175,3 +175,18 @@ def test_linear_of_few_rows_and_of_more(gpu, K, M, dtype):
         whole = run(sizes[0])
         for n in sizes[1:]:
             assert all(torch.equal(a[:n], c) for a, c in zip(whole, run(n))), n
+
+
+def test_a_random_state_that_moved_on_is_not_taken_for_the_one_that_was_drawn_from(gpu):
+    """a layer's own state handed to another as its `rng`: backward needs it as it was"""
+    import occuseg_amd.sparseconvnet as scn
+    a, b = scn.Dropout(0.5).to(gpu), scn.Dropout(0.5).to(gpu)
+    x = torch.ones(64, 64, device=gpu, requires_grad=True)
+    y = a(scn.SparseConvNetTensor(x), rng=b.rng_state).features
+    b(scn.SparseConvNetTensor(x.detach()))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y = a(scn.SparseConvNetTensor(x), rng=b.rng_state.clone()).features
+    b(scn.SparseConvNetTensor(x.detach()))
+    y.sum().backward()
+    assert torch.equal(x.grad, y.detach())
