@@ -48,7 +48,7 @@ __device__ __forceinline__ void store_some(T *p, const Pack<T, V> &v, int n) {
 // ------------------------------------------------------------------- dropout ---
 // Every element read and written once; the mask is made of the counter.  A thread keeps its planes -- Q quads -- and walks the
 // sites, `rows` of a step at a time: the products of the counter that belong to the planes are made once.  Four rows are requested
-// before the first is used.  HBM bound: 601,674 x 128 bf16 take 62 us = 5.0 TB/s, a copy of as many bytes 57.
+// before the first is used.  HBM bound: 601,674 x 128 bf16 take 65 us = 4.7 TB/s, a copy of as many bytes 58.
 template <class T, int Q, bool WHOLE>
 __global__ void __launch_bounds__(256)
     k_dropout(const T *x, int64_t ldx, T *y, int64_t N, int C, int items, int rows, uint32_t threshold, float scale, const int64_t *rng) {
@@ -143,7 +143,7 @@ __device__ __forceinline__ int16_t short_float(float v) {
   const bool negative = v < 0;
   const uint32_t b = __builtin_bit_cast(uint32_t, fabsf(v) * (negative ? 0x1p-93f : 0x1p-120f));
   const int shift = negative ? 13 : 11;
-  return v == v ? (int16_t)((b + (1u << shift >> 1)) >> shift | (negative ? 0x8000u : 0u)) : (int16_t)0x7fff;
+  return (int16_t)(min((b + (1u << shift >> 1)) >> shift, 0x7fffu) | (negative ? 0x8000u : 0u));  // (only NaN, not below 0, reaches 0x7fff)
 }
 __device__ __forceinline__ float short_float_value(int16_t q) {
   const bool negative = q < 0;
@@ -164,7 +164,7 @@ __device__ __forceinline__ float times_factor(float dy, Q q, float leak) {
 // z of 16-bit features as two operands, z rounded and what that lost, whose products are added one behind the other: what is lost is the
 // square of a rounding (fp16: and what lies below its subnormal numbers).  One operand alone doubles the variance of the gradients' own
 // rounding (bf16 dx and dW off by 2.4e-3 instead of 1.7e-3, relative), and the matrix pipe waits for memory either way: 177,001 x 128 to
-// 512, bf16, GELU, dx 94 us with one and with two, dW 108 and 109.  (Where rounding would give infinity: the largest number, and the rest
+// 512, bf16, GELU, one call behind the other, dx 94 us with one and with two, dW 108 and 109.  (Where rounding would give infinity: the largest number, and the rest
 // beside it; infinity and NaN are in the rest.)
 template <class T>
 __device__ __forceinline__ void split(float z, T &rounded, T &rest) {
@@ -220,13 +220,15 @@ constexpr int lin_piece_bytes(int nt, bool packed) { return packed ? 16 * (lin_p
 // A workgroup holds the weights of NT x 16 output planes in LDS -- all of K, once, if they fit (STAY): then it has a CU to itself and
 // its waves take 32-row tiles without a barrier -- else `chunk_groups` at a time, and its waves keep together.  Tiles are taken from a
 // counter in LDS: the older of the waves on a SIMD come first at its matrix pipe and take 15 us a tile where the youngest take 37
-// (200,000 x 128 to 128, fp32), so that equal shares end at 50 to 85 us.
+// (200,000 x 128 to 128, fp32), so that equal shares would end at 50 to 85 us.
 // Beside fp32 MFMAs a vector instruction costs 8 or more of the matrix pipe's cycles, and the epilogue alone fills half the time of
 // a 16-bit layer: addresses are a scalar base and one 32-bit offset a lane for all tiles, the bias is what the accumulators start
 // from, and the epilogue is compiled for each activation, with and without dropout and factors.
-// Measured: 601,674 x 64 to 20, fp32, 40 us = 5.1 TB/s; 177,001 x 64 to 128, fp32, GELU, dropout, residual and factors, 66 us = 4.8 TB/s
-// (forward), 42 us = 5.4 TB/s (dx); 177,001 x 128 to 512, bf16, GELU, dropout and factors, 118 us = 3.4 TB/s (forward: some 37 vector
-// instructions an output), 92 us = 4.4 TB/s (dx; a plain sum reads 4.0 to 4.9); fp32 that is not bound by memory: 200,000 x 128 to 128 80 us = 82 TFLOP/s.
+// Measured, medians with inputs that are not cached: 601,674 x 64 to 20, fp32, 45 us = 4.5 TB/s; 177,001 x 64 to 128, fp32, GELU, dropout,
+// residual and factors, 68 us = 4.7 TB/s (forward), 45 us = 5.1 TB/s (dx); 177,001 x 128 to 512, GELU, dropout and factors, bf16 140 us =
+// 2.9 TB/s (forward: some 43 vector instructions an output), 109 us = 3.7 TB/s (dx), fp16 154 and 113 us; without activation and dropout,
+// bf16, 59 us = 3.8 TB/s and 62 us = 3.6 TB/s; fp32 that is not bound by memory: 200,000 x 128 to 128 96 us = 68 TFLOP/s, 100,000 x 512 to
+// 512 538 us = 97 TFLOP/s.
 template <class T, int NT, int MODE, int X, bool STAY>
 __global__ void __launch_bounds__(64 * lin_waves(NT, STAY), NT == 8 || !STAY ? 3 : 4) k_linear(LinearArgs a) {
   constexpr int WAVES = lin_waves(NT, STAY), THREADS = 64 * WAVES;
@@ -584,8 +586,9 @@ __global__ void __launch_bounds__(1024) k_linear_few(LinearArgs a) {
 // loaded element by element (the last rows of the last slice).
 // Workgroup (slice, tile): four waves take the slice's row steps in turn, join through LDS and write one slab; slabs are added by
 // k_linear_dw_join in slice order.
-// HBM bound, with the join: 177,001 x 64 to 128, fp32, with factors 52 us = 4.3 TB/s; 128 to 512, bf16, 104 us = 3.9 TB/s (without
-// factors 53 us = 4.3 TB/s).  Few sites: a step's latency three times over, the waves' join and the slabs, 18 us for 50,001 x 35 to 77.
+// HBM bound; medians with inputs that are not cached, without the join's 4 to 8 us: 177,001 x 64 to 128, fp32, with factors 50 us = 4.5
+// TB/s; 128 to 512, bf16, 105 us = 3.9 TB/s (without factors 62 us = 3.6 TB/s).  Few sites: a step's latency three times over and the
+// waves' join, 16 us for 50,001 x 35 to 77, fp16, and 4 for the slabs.
 struct DwArgs {
   const void *x, *dy, *factor;
   int64_t ldx, ld_dy, N;
@@ -795,7 +798,7 @@ static int by_type(int dtype, F &&f) {
 }
 
 // The forward pass's weights come as [n_in, n_out].  Workgroups whose weights stay in LDS scatter them there themselves: 5,000 to 200,000
-// sites x 64..128 to 20..256 planes take 1.5 to 5 us less than with a launch (2.5 us) that lays them out as [n_out, n_in] first.  That
+// sites x 64..128 to 20..256 planes take 1.5 to 5 us less than with a launch (2.5 us where they are cached, 5 where not) that lays them out as [n_out, n_in] first.  That
 // launch is needed where the weights do not stay and every workgroup fetches all of them (four column tiles of 22 k-groups do), and
 // for the eight column tiles that many outputs of 16-bit types are worth (200,000 x 128 to 256, bf16: 40.7 us, 47.6 without; to 128 30.2
 // and 29.4; 600,000 x 448 to 256, where eight do not stay and four do, 308 and 338).

@@ -41,8 +41,9 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r) {
 // One reciprocal and one exponential of the hardware each (1 ulp; an exponent x is off by |x| 2^-24, where e^x is as small).  The tail
 // 1 - Phi(t), t >= 0, is the density phi(t) -- which the slope needs too -- times a smooth function of t, here a polynomial in
 // s = 1 / (1 + c t) without a constant term, fitted to (1 - Phi) / phi over t <= 40 by iteratively reweighted least squares.  Largest
-// relative error of z Phi(z) over |z| <= 9, in fp32: 4.8e-7 with nine terms (float features), 2.9e-6 with seven (fp16, whose half
-// step is 4.9e-4 at its finest), 6.1e-5 with five (bf16: 3.9e-3).
+// relative error of z Phi(z) as these steps compute it in fp32, |z| <= 3 and |z| <= 9 (where the exponent's rounding counts: up to 58):
+// nine terms (float features) 6.5e-7 and 3.8e-6, seven (fp16, whose half step is 4.9e-4) 3.2e-6 and 4.4e-6, five (bf16: 3.9e-3) 6.0e-5
+// and 6.1e-5; z / (1 + e^-z), |z| <= 16: 5.5e-7.
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 template <class T> constexpr int act_terms() { return sizeof(T) == 4 ? 9 : std::is_same<T, __bf16>::value ? 5 : 7; }
 

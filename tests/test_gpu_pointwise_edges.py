@@ -190,3 +190,30 @@ def test_a_random_state_that_moved_on_is_not_taken_for_the_one_that_was_drawn_fr
     b(scn.SparseConvNetTensor(x.detach()))
     y.sum().backward()
     assert torch.equal(x.grad, y.detach())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("N,K,M", [(3, 5, 4), (200, 70, 33), (300, 64, 128)])
+def test_slopes_that_are_nan_reach_the_gradients(gpu, dtype, activation, N, K, M):
+    """a row of NaN, of either sign: its row of dx, and all of dW and db; the other rows of dx are as without it"""
+    t = TYPES[dtype]
+    x, w, b, dy = rnd(61, N, K).to(t), (rnd(62, K, M) * K ** -0.5).to(t), (0.1 * rnd(63, M)).to(t), rnd(64, N, M).to(t)
+    want = run_linear(gpu, x, w, b, None, activation, 1, 0.0, None, dy)[1]
+    for bad in (float("nan"), -float("nan")):
+        x[N // 2] = bad
+        y, dx, dw, db = run_nan(gpu, x, w, b, activation, dy)
+        rows = torch.arange(N) != N // 2
+        assert y[N // 2].isnan().all() and dx[N // 2].isnan().all() and dw.isnan().all() and db.isnan().all()
+        assert torch.equal(dx[rows], want[rows])
+
+
+def run_nan(gpu, x, w, b, activation, dy):
+    import occuseg_amd.sparseconvnet as scn
+    m = scn.FusedNetworkInNetwork(w.size(0), w.size(1), True, activation).to(gpu).to(x.dtype)
+    with torch.no_grad():
+        m.weight.copy_(w)
+        m.bias.copy_(b)
+    xg = x.to(gpu).requires_grad_(True)
+    y = m(scn.SparseConvNetTensor(xg)).features
+    return [y] + list(torch.autograd.grad(y, [xg, m.weight, m.bias], dy.to(gpu)))
