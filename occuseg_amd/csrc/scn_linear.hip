@@ -226,7 +226,7 @@ constexpr int lin_piece_bytes(int nt, bool packed) { return packed ? 16 * (lin_p
 // from, and the epilogue is compiled for each activation, with and without dropout and factors.
 // Measured, medians with inputs that are not cached: 601,674 x 64 to 20, fp32, 45 us = 4.5 TB/s; 177,001 x 64 to 128, fp32, GELU, dropout,
 // residual and factors, 68 us = 4.7 TB/s (forward), 45 us = 5.1 TB/s (dx); 177,001 x 128 to 512, GELU, dropout and factors, bf16 140 us =
-// 2.9 TB/s (forward: some 43 vector instructions an output), 109 us = 3.7 TB/s (dx), fp16 154 and 113 us; without activation and dropout,
+// 2.9 TB/s (forward: some 31 vector instructions an output), 109 us = 3.7 TB/s (dx), fp16 148 and 111 us; without activation and dropout,
 // bf16, 59 us = 3.8 TB/s and 62 us = 3.6 TB/s; fp32 that is not bound by memory: 200,000 x 128 to 128 96 us = 68 TFLOP/s, 100,000 x 512 to
 // 512 538 us = 97 TFLOP/s.
 template <class T, int NT, int MODE, int X, bool STAY>
