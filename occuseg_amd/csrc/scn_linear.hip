@@ -164,8 +164,8 @@ __device__ __forceinline__ float times_factor(float dy, Q q, float leak) {
 // z of 16-bit features as two operands, z rounded and what that lost, whose products are added one behind the other: what is lost is the
 // square of a rounding (fp16: and what lies below its subnormal numbers).  One operand alone doubles the variance of the gradients' own
 // rounding (bf16 dx and dW off by 2.4e-3 instead of 1.7e-3, relative), and the matrix pipe waits for memory either way: 177,001 x 128 to
-// 512, bf16, GELU, one call behind the other, dx 94 us with one and with two, dW 108 and 109.  (Where rounding would give infinity: the largest number, and the rest
-// beside it; infinity and NaN are in the rest.)
+// 512, bf16, GELU, one call behind the other, dx 94 us with one and with two, dW 108 and 109.  (Where rounding would give infinity: the
+// largest number, and the rest beside it; infinity and NaN are in the rest.)
 template <class T>
 __device__ __forceinline__ void split(float z, T &rounded, T &rest) {
   constexpr float most = std::is_same<T, __bf16>::value ? 0x1.fep127f : 65504.f;
@@ -798,8 +798,8 @@ static int by_type(int dtype, F &&f) {
 }
 
 // The forward pass's weights come as [n_in, n_out].  Workgroups whose weights stay in LDS scatter them there themselves: 5,000 to 200,000
-// sites x 64..128 to 20..256 planes take 1.5 to 5 us less than with a launch (2.5 us where they are cached, 5 where not) that lays them out as [n_out, n_in] first.  That
-// launch is needed where the weights do not stay and every workgroup fetches all of them (four column tiles of 22 k-groups do), and
+// sites x 64..128 to 20..256 planes take 1.5 to 5 us less than with a launch (2.5 us where they are cached, 5 where not) that lays them out
+// as [n_out, n_in] first.  That launch is needed where the weights do not stay and every workgroup fetches all of them (four column tiles of 22 k-groups do), and
 // for the eight column tiles that many outputs of 16-bit types are worth (200,000 x 128 to 256, bf16: 40.7 us, 47.6 without; to 128 30.2
 // and 29.4; 600,000 x 448 to 256, where eight do not stay and four do, 308 and 338).
 constexpr int64_t LIN_WIDE = (int64_t)1 << 25;  // sites x n_out
