@@ -799,9 +799,9 @@ static int by_type(int dtype, F &&f) {
 
 // The forward pass's weights come as [n_in, n_out].  Workgroups whose weights stay in LDS scatter them there themselves: 5,000 to 200,000
 // sites x 64..128 to 20..256 planes take 1.5 to 5 us less than with a launch (2.5 us where they are cached, 5 where not) that lays them out
-// as [n_out, n_in] first.  That launch is needed where the weights do not stay and every workgroup fetches all of them (four column tiles of 22 k-groups do), and
-// for the eight column tiles that many outputs of 16-bit types are worth (200,000 x 128 to 256, bf16: 40.7 us, 47.6 without; to 128 30.2
-// and 29.4; 600,000 x 448 to 256, where eight do not stay and four do, 308 and 338).
+// as [n_out, n_in] first.  That launch is needed where the weights do not stay and every workgroup fetches all of them (four column tiles
+// of 22 k-groups do), and for the eight column tiles that many outputs of 16-bit types are worth (200,000 x 128 to 256, bf16: 40.7 us,
+// 47.6 without; to 128 30.2 and 29.4; 600,000 x 448 to 256, where eight do not stay and four do, 308 and 338).
 constexpr int64_t LIN_WIDE = (int64_t)1 << 25;  // sites x n_out
 constexpr int LIN_LDS = 163840;  // of a CU
 constexpr int LIN_FEW = 4;  // up to this many sites: k_linear_few
